@@ -71,6 +71,10 @@ _SIGS = {
     "jllm_adjust_logits": [_P, _I, _P, _P, _I, _F, _F, _F, _P, _P, _I, _P],
     "jllm_token_logprobs": [_P, _I, _I, _I, _P, _I, _P, _P, _P, _P],
     "jllm_copy_words": [_P, _P, _L, _P],
+    "jllm_quantize_rows": [_P, _I, _I, _I, _I, _P, _I, _P, _P],
+    "jllm_dequantize_rows": [_P, _I, _P, _I, _I, _P, _I, _I, _P],
+    "jllm_rmsnorm_int8": [_P, _I, _P, _I, _I, _P, _I, _I, _I, _P, _I, _F, _P, _I, _P, _P],
+    "jllm_gemm_int8": [_P, _I, _P, _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P],
     "jllm_latent_prepare": [_P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _P, _P, _P, _P, _I, _P, _P],
     "jllm_latent_heads_generic": [_P, _I, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P],
     "jllm_latent_attention_generic": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P],
@@ -643,6 +647,178 @@ def gemm(a: torch.Tensor, w: torch.Tensor, *, w2: Optional[torch.Tensor] = None,
         _count("general", "jllm_gemm_generic")
     _call("jllm_gemm_generic", _ptr(a), _code(a.dtype), a.stride(0), _ptr(w), _ptr(w2), _code(w.dtype), _ptr(bias),
           _code(bias.dtype) if bias is not None else F32, _ptr(out), _code(out.dtype), out.stride(0), M, N, K,
+          int(epilogue), float(gate_limit), _stream())
+    return out
+
+
+# ------------------------------------------------------------------------------------------------ rows of 8-bit integers
+
+
+class Int8Rows:
+    """Rows of 8-bit integers: ``q`` (int8 [n, width], rows contiguous, any distance apart) and one fp32 ``scale`` per row [n]; row r
+    stands for ``q[r] * scale[r]``. Activations are such rows by token, a weight [N, K] by output channel. Made by
+    ``quantize_rows`` and ``rmsnorm_int8``, or from tensors at hand."""
+
+    __slots__ = ("q", "scale")
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor):
+        self.q, self.scale = q, scale
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+    def tensor(self, dtype: torch.dtype) -> torch.Tensor:
+        """The values that the rows stand for, rounded once to ``dtype``."""
+        _int8_rows(self, "rows")
+        code = _code(dtype)
+        _here(self.q, self.scale)
+        n, width = self.q.shape
+        out = activation_rows(n, width, dtype, self.q.device)
+        if n and width:
+            _call("jllm_dequantize_rows", _ptr(self.q), _distance(self.q), _ptr(self.scale), n, width, _ptr(out), code, _distance(out), _stream())
+        return out
+
+
+INT8_MOST_INPUTS = 131071  # of a product: 128^2 times as many stay below 2^31, so every sum is exact
+
+
+def _distance(t: torch.Tensor) -> int:
+    """Entries between the rows of a 2-D tensor; a single row's stride says nothing."""
+    apart = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if apart >= 1 << 31 or t.shape[0] >= 1 << 31:
+        raise KernelError(f"the kernels take fewer than 2^31 rows, less than 2^31 entries apart; got {tuple(t.shape)}, strides {t.stride()}")
+    return apart
+
+
+def _here(*tensors) -> None:
+    """All on the current GPU, on whose stream the launch goes."""
+    _dev(*tensors)
+    now = _raw_device()
+    for t in tensors:
+        if t is not None and t.get_device() != now:
+            raise KernelError(f"the engine's kernels run on the current GPU (cuda:{now}); got a tensor on {t.device}")
+
+
+def _apart(t: torch.Tensor, what: str) -> None:
+    """Rows that are written: none over another."""
+    if _distance(t) < t.shape[1]:
+        raise KernelError(f"{what} must have rows of their own, got shape {tuple(t.shape)} strides {t.stride()}")
+
+
+def _int8_rows(rows: Int8Rows, what: str) -> None:
+    if not isinstance(rows, Int8Rows):
+        raise KernelError(f"{what} must be Int8Rows, got {type(rows).__name__}")
+    if rows.q.dtype != torch.int8:
+        raise KernelError(f"{what} must be int8, got {rows.q.dtype}")
+    _rows2d(rows.q, what)
+    if rows.scale.dtype != torch.float32 or rows.scale.dim() != 1 or rows.scale.shape[0] != rows.q.shape[0] or not rows.scale.is_contiguous():
+        raise KernelError(f"{what}: the scales must be a contiguous fp32 tensor with one entry per row ({rows.q.shape[0]}), got "
+                          f"{rows.scale.dtype} {tuple(rows.scale.shape)}")
+
+
+def _vector(t: Optional[torch.Tensor], n: int, what: str) -> None:
+    if t is not None and (t.numel() != n or not t.is_contiguous()):
+        raise KernelError(f"{what} has {t.numel()} entries for rows of {n}")
+
+
+def _new_int8_rows(n: int, width: int, device) -> Int8Rows:
+    return Int8Rows(torch.empty((n, width), dtype=torch.int8, device=device), torch.empty((n,), dtype=torch.float32, device=device))
+
+
+def quantize_rows(x: torch.Tensor) -> Int8Rows:
+    """Rows of ``x`` (fp32 or bf16 [n, width], any distance apart) as 8-bit integers: scale = max |x| / 127, q = x * (127 / max |x|)
+    rounded to the nearest whole number, halves to even. A row of zeros has scale 0; one with a NaN or an infinity has scale NaN
+    and zeros, so that what is computed from it is NaN. For activations in front of ``gemm_int8``, and for a weight [N, K] at load."""
+    _rows2d(x, "quantize_rows input")
+    dtype = _code(x.dtype)
+    n, width = x.shape
+    if width == 0:
+        raise KernelError("quantize_rows: rows without entries have no scale")
+    _here(x)
+    out = _new_int8_rows(n, width, x.device)
+    if n:
+        _call("jllm_quantize_rows", _ptr(x), dtype, _distance(x), n, width, _ptr(out.q), _distance(out.q), _ptr(out.scale), _stream())
+    return out
+
+
+def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None) -> Int8Rows:
+    """RMSNorm of fp32 rows of ``x`` with ``gain`` as 8-bit rows for ``gemm_int8`` (scales and rounding as ``quantize_rows``; the norm
+    itself is not rounded in between). With ``add`` (fp32 or bf16, of x's shape), what a sublayer leaves, the norm is that of
+    ``x + add``, and the sum goes to ``out`` (fp32; not given: into ``x``, the residual stream)."""
+    if x.dtype != torch.float32:
+        raise KernelError("rmsnorm_int8 takes fp32 rows")
+    _rows2d(x, "rmsnorm_int8 input")
+    n, width = x.shape
+    if width == 0:
+        raise KernelError("rmsnorm_int8: rows without entries have no norm")
+    _vector(gain, width, "rmsnorm_int8 gain")
+    if add is None:
+        if out is not None:
+            raise KernelError("rmsnorm_int8: a place for the sum without rows to add")
+    else:
+        _rows2d(add, "rmsnorm_int8 rows to add")
+        if add.shape != x.shape:
+            raise KernelError(f"rmsnorm_int8: rows to add {tuple(add.shape)} for {tuple(x.shape)}")
+        out = x if out is None else out
+        _rows2d(out, "rmsnorm_int8 sum")
+        if out.dtype != torch.float32 or out.shape != x.shape:
+            raise KernelError(f"rmsnorm_int8: the sum goes to an fp32 tensor of x's shape, got {out.dtype} {tuple(out.shape)}")
+        _apart(out, "rmsnorm_int8 sum")
+    gain_code, add_code = _code(gain.dtype), _code(add.dtype) if add is not None else F32
+    _here(x, gain, add, out)
+    rows = _new_int8_rows(n, width, x.device)
+    if n:
+        _call("jllm_rmsnorm_int8", _ptr(x), _distance(x), _ptr(add), add_code, _distance(add) if add is not None else 0, _ptr(out),
+              _distance(out) if out is not None else 0, n, width, _ptr(gain), gain_code, float(eps), _ptr(rows.q), _distance(rows.q), _ptr(rows.scale),
+              _stream())
+    return rows
+
+
+def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None, epilogue: int = EPI_STORE,
+              gate: int = 0, gate_limit: float = 0.0) -> torch.Tensor:
+    """out[m, n] = a.scale[m] * w.scale[n] * sum_k a.q[m, k] * w.q[n, k] (+ bias[n]): a product of 8-bit rows with a weight's output
+    channels. The sums are whole numbers and exact (up to 131,071 inputs), so a row has the same bits whatever rows stand
+    beside it. Epilogues and gate functions as in ``gemm``: EPI_STORE writes ``out_dtype`` (bf16 where nothing is said), EPI_ADD adds into
+    the fp32 ``out``, EPI_GATED writes gate(a w + bias, a w2)."""
+    _int8_rows(a, "gemm_int8 input")
+    _int8_rows(w, "gemm_int8 weight")
+    M, K = a.q.shape
+    N = w.q.shape[0]
+    if w.q.shape[1] != K:
+        raise KernelError(f"gemm_int8: input rows have {K} entries, weight rows {w.q.shape[1]}")
+    if not 0 < K <= INT8_MOST_INPUTS:
+        raise KernelError(f"gemm_int8: rows of {K} entries (1 to {INT8_MOST_INPUTS}: beyond, the sums could leave 32 bits)")
+    if epilogue not in (EPI_STORE, EPI_ADD, EPI_GATED) or (epilogue == EPI_GATED) != (w2 is not None):
+        raise KernelError("gemm_int8: the gated epilogue takes exactly two weights")
+    if w2 is not None:
+        _int8_rows(w2, "gemm_int8 second weight")
+        if w2.q.shape != w.q.shape:
+            raise KernelError("gemm_int8: the two weights of the gated epilogue must agree in shape")
+    if gate and (epilogue != EPI_GATED or not 0 < gate < (1 << 20)):
+        raise KernelError(f"gemm_int8: gate function {gate} without the gated epilogue")
+    _vector(bias, N, "gemm_int8 bias")
+    bias_code = _code(bias.dtype) if bias is not None else F32
+    if epilogue == EPI_ADD and (out is None or out.dtype != torch.float32):
+        raise KernelError("gemm_int8: the accumulate epilogue needs an fp32 output to add into")
+    if out is not None:
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise KernelError(f"gemm_int8: output is {out.dtype}, asked for {out_dtype}")
+        _rows2d(out, "gemm_int8 output")
+        if out.shape[0] != M or out.shape[1] != N:
+            raise KernelError(f"gemm_int8: output is {tuple(out.shape)}, expected {(M, N)}")
+        _apart(out, "gemm_int8 output")
+    out_code = _code(out.dtype if out is not None else out_dtype or torch.bfloat16)
+    _here(a.q, a.scale, w.q, w.scale, *((w2.q, w2.scale) if w2 is not None else ()), bias, out)
+    if out is None:
+        out = activation_rows(M, N, out_dtype or torch.bfloat16, a.q.device)
+    if M == 0 or N == 0:
+        return out
+    epilogue = int(epilogue) | (int(gate) << 8)  # the kernels take it apart again and refuse what they do not have
+    _call("jllm_gemm_int8", _ptr(a.q), _distance(a.q), _ptr(a.scale), _ptr(w.q), _distance(w.q), _ptr(w.scale), _ptr(w2.q) if w2 else None,
+          _distance(w2.q) if w2 else 0, _ptr(w2.scale) if w2 else None, _ptr(bias), bias_code, _ptr(out), out_code, _distance(out), M, N, K,
           int(epilogue), float(gate_limit), _stream())
     return out
 

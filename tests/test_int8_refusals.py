@@ -1,0 +1,91 @@
+"""What the operators on rows of 8-bit integers refuse, and with which words, before anything is launched (no GPU)."""
+import pytest
+import torch
+
+from jllm_serve_amd.kernels import ops
+
+
+def rows(n=4, width=32, dtype=torch.int8, scales=None):
+    return ops.Int8Rows(torch.zeros((n, width), dtype=dtype), torch.ones(n if scales is None else scales))
+
+
+def refused(words, call, *args, **kw):
+    with pytest.raises(ops.KernelError) as e:
+        call(*args, **kw)
+    assert words in str(e.value), str(e.value)
+
+
+def test_no_cpu_path():
+    refused("GPU only", ops.quantize_rows, torch.zeros(3, 8))
+    refused("GPU only", ops.rmsnorm_int8, torch.zeros(3, 8), torch.zeros(8), 1e-6)
+    refused("GPU only", ops.gemm_int8, rows(), rows(6))
+    refused("GPU only", rows().tensor, torch.float32)
+
+
+def test_quantize_rows():
+    refused("contiguous rows", ops.quantize_rows, torch.zeros(8))
+    refused("contiguous rows", ops.quantize_rows, torch.zeros(8, 4).t())
+    refused("float32 or bfloat16", ops.quantize_rows, torch.zeros(3, 8, dtype=torch.float16))
+    refused("without entries", ops.quantize_rows, torch.zeros(3, 0))
+
+
+def test_int8_rows():
+    refused("must be int8", rows(dtype=torch.uint8).tensor, torch.float32)
+    refused("one entry per row", rows(scales=3).tensor, torch.float32)
+    refused("one entry per row", ops.Int8Rows(torch.zeros((4, 8), dtype=torch.int8), torch.ones(4, dtype=torch.float64)).tensor, torch.float32)
+    refused("one entry per row", ops.Int8Rows(torch.zeros((4, 8), dtype=torch.int8), torch.ones(4, 1)).tensor, torch.float32)
+    refused("contiguous fp32", ops.Int8Rows(torch.zeros((4, 8), dtype=torch.int8), torch.ones(8)[::2]).tensor, torch.float32)
+    refused("contiguous rows", ops.Int8Rows(torch.zeros((8, 4), dtype=torch.int8).t(), torch.ones(4)).tensor, torch.float32)
+    refused("float32 or bfloat16", rows().tensor, torch.float16)
+
+
+def test_rmsnorm_int8():
+    x, g = torch.zeros(3, 8), torch.ones(8)
+    refused("fp32 rows", ops.rmsnorm_int8, x.bfloat16(), g, 1e-6)
+    refused("contiguous rows", ops.rmsnorm_int8, torch.zeros(8, 3).t(), g, 1e-6)
+    refused("no norm", ops.rmsnorm_int8, torch.zeros(3, 0), torch.ones(0), 1e-6)
+    refused("gain has 7", ops.rmsnorm_int8, x, torch.ones(7), 1e-6)
+    refused("float32 or bfloat16", ops.rmsnorm_int8, x, g.half(), 1e-6)
+    refused("without rows to add", ops.rmsnorm_int8, x, g, 1e-6, out=torch.zeros(3, 8))
+    refused("rows to add", ops.rmsnorm_int8, x, g, 1e-6, add=torch.zeros(2, 8))
+    refused("float32 or bfloat16", ops.rmsnorm_int8, x, g, 1e-6, add=x.half())
+    refused("fp32 tensor of x's shape", ops.rmsnorm_int8, x, g, 1e-6, add=x, out=x.bfloat16())
+    refused("fp32 tensor of x's shape", ops.rmsnorm_int8, x, g, 1e-6, add=x, out=torch.zeros(3, 9))
+    refused("rows of their own", ops.rmsnorm_int8, x, g, 1e-6, add=x, out=torch.zeros(1, 8).expand(3, 8))
+    refused("rows of their own", ops.rmsnorm_int8, torch.zeros(1, 8).expand(3, 8), g, 1e-6, add=x)
+    refused("rows of their own", ops.rmsnorm_int8, x, g, 1e-6, add=x, out=torch.zeros(30).as_strided((3, 8), (7, 1)))
+
+
+def test_gemm_int8():
+    a, w = rows(4), rows(6)
+    refused("must be Int8Rows", ops.gemm_int8, a.q, w)
+    refused("must be Int8Rows", ops.gemm_int8, a, w.q)
+    refused("must be Int8Rows", ops.gemm_int8, a, w, w2=w.q, epilogue=ops.EPI_GATED)
+    refused("input rows have 32", ops.gemm_int8, a, rows(6, 31))
+    refused("rows of 0", ops.gemm_int8, rows(4, 0), rows(6, 0))
+    refused("leave 32 bits", ops.gemm_int8, rows(1, 131072), rows(1, 131072))
+    refused("exactly two weights", ops.gemm_int8, a, w, w2=w)
+    refused("exactly two weights", ops.gemm_int8, a, w, epilogue=ops.EPI_GATED)
+    refused("exactly two weights", ops.gemm_int8, a, w, epilogue=3)
+    refused("agree in shape", ops.gemm_int8, a, w, w2=rows(5), epilogue=ops.EPI_GATED)
+    refused("without the gated", ops.gemm_int8, a, w, gate=1)
+    refused("without the gated", ops.gemm_int8, a, w, w2=w, epilogue=ops.EPI_GATED, gate=1 << 20)
+    refused("bias has 5", ops.gemm_int8, a, w, bias=torch.zeros(5))
+    refused("bias has 6", ops.gemm_int8, a, w, bias=torch.zeros(12)[::2])
+    refused("float32 or bfloat16", ops.gemm_int8, a, w, bias=torch.zeros(6, dtype=torch.float16))
+    refused("fp32 output", ops.gemm_int8, a, w, epilogue=ops.EPI_ADD)
+    refused("fp32 output", ops.gemm_int8, a, w, out=torch.zeros(4, 6).bfloat16(), epilogue=ops.EPI_ADD)
+    refused("expected (4, 6)", ops.gemm_int8, a, w, out=torch.zeros(4, 7))
+    refused("asked for", ops.gemm_int8, a, w, out=torch.zeros(4, 6), out_dtype=torch.bfloat16)
+    refused("rows of their own", ops.gemm_int8, a, w, out=torch.zeros(1, 6).expand(4, 6))
+    refused("contiguous rows", ops.gemm_int8, a, w, out=torch.zeros(6, 4).t())
+    refused("float32 or bfloat16", ops.gemm_int8, a, w, out_dtype=torch.float16)
+    refused("float32 or bfloat16", ops.gemm_int8, a, w, out=torch.zeros(4, 6).half())
+    refused("one entry per row", ops.gemm_int8, rows(4, scales=5), w)
+
+
+def test_a_single_row_may_have_any_stride():
+    """A row alone has no distance to the next: it is not refused for the stride it happens to have."""
+    assert ops._distance(torch.zeros(8, 1).t()) == 8
+    ops._apart(torch.zeros(8, 1).t(), "row")
+    refused("2^31", ops._distance, torch.zeros(0, dtype=torch.int8).as_strided((2, 0), (1 << 31, 1)))
