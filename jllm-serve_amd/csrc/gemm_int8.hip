@@ -11,16 +11,14 @@
 
 struct Gemm8Args {
   const signed char *A, *W, *W2;
-  Int8Scales scales;
-  const void* bias;
-  void* out;
-  int lda, ldw, ldw2, bias_dtype, out_dtype, ldo, M, N, K, epilogue;
-  GateSpec gate;
+  int lda, ldw, ldw2, K;
+  Int8Epilogue end;
 };
 
 template <bool GATED>
 __global__ __launch_bounds__(256) void gemm_int8_kernel(Gemm8Args p) {
   constexpr int TBM = 64, TBN = 64, COLS = GATED ? 32 : 64;
+  const int M = p.end.M, N = p.end.N;
   __shared__ __align__(16) unsigned char lds[2][(TBM + TBN) * G8_PITCH];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
   const int m0 = blockIdx.y * TBM, n0 = blockIdx.x * COLS;
@@ -31,11 +29,11 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(Gemm8Args p) {
   for (int c = 0; c < 4; ++c) {
     const int r = (tid >> 3) + (c & 1) * 32;
     if (c < 2) {
-      from[c] = p.A + (size_t)min(m0 + r, p.M - 1) * p.lda;
+      from[c] = p.A + (size_t)min(m0 + r, M - 1) * p.lda;
     } else {  // gated: of a wave's two blocks of 16 the first is gate rows, the second the up rows of the same outputs
       const bool second = GATED && (r & 16);
       const int n = GATED ? n0 + (r >> 5) * 16 + (r & 15) : n0 + r;
-      from[c] = (second ? p.W2 : p.W) + (size_t)min(n, p.N - 1) * (second ? p.ldw2 : p.ldw);
+      from[c] = (second ? p.W2 : p.W) + (size_t)min(n, N - 1) * (second ? p.ldw2 : p.ldw);
     }
   }
   u32x4 held[4];
@@ -82,30 +80,7 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(Gemm8Args p) {
     }
     if (t + 1 < stages) put((t + 1) & 1);
   }
-  // (tile_epilogue stores runs in pairs: gated, a wave has one run of outputs, so both blocks' sums are combined here)
-  if constexpr (GATED) {
-    const int n = n0 + wn * 16 + (lane >> 4) * 4;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int m = m0 + wm * 32 + i * 16 + (lane & 15);
-      if (m >= p.M) continue;
-      const float sa = p.scales.a[m];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (n + c >= p.N) continue;
-        float z = ((float)acc[i][0][c] * sa) * p.scales.w[n + c];
-        if (p.bias) z += p.bias_dtype == JLLM_BF16 ? ldf((const bf16_t*)p.bias, n + c) : ldf((const float*)p.bias, n + c);
-        const float y = gated<true>(z, ((float)acc[i][1][c] * sa) * p.scales.w2[n + c], p.gate);
-        const size_t o = (size_t)m * p.ldo + n + c;
-        if (p.out_dtype == JLLM_BF16)
-          stf((bf16_t*)p.out, o, y);
-        else
-          stf((float*)p.out, o, y);
-      }
-    }
-  } else {
-    int8_epilogue<false, 2, 2, TBM, TBN>(acc, lane, wm, wn, m0, n0, p.scales, p.bias, p.bias_dtype, p.out, p.out_dtype, p.ldo, p.M, p.N, p.epilogue, p.gate);
-  }
+  int8_epilogue<GATED, 2, 2>(acc, lane, wm, wn, m0, n0, p.end);
 }
 
 extern "C" int jllm_gemm_int8(const void* A, int lda, const float* a_scale, const void* W, int ldw, const float* w_scale, const void* W2, int ldw2,
@@ -119,8 +94,8 @@ extern "C" int jllm_gemm_int8(const void* A, int lda, const float* a_scale, cons
   if (lda < 0 || ldw < 0 || ldw2 < 0 || ldo < N) JLLM_FAIL("gemm_int8: rows %d, %d and %d apart", lda, ldw, ldo);
   const dim3 grid(W2 ? (N + 31) / 32 : (N + 63) / 64, (M + 63) / 64);
   if (grid.y > 65535) JLLM_FAIL("gemm_int8: %d rows are more than a grid takes", M);
-  const Gemm8Args a{(const signed char*)A, (const signed char*)W, (const signed char*)W2, {a_scale, w_scale, w2_scale}, bias, out, lda, ldw, ldw2,
-                    bias_dtype, out_dtype, ldo, M, N, K, epilogue, gs};
+  const Gemm8Args a{(const signed char*)A, (const signed char*)W, (const signed char*)W2, lda, ldw, ldw2, K,
+                    {{a_scale, w_scale, w2_scale}, bias, out, bias_dtype, out_dtype, ldo, M, N, epilogue, gs}};
   if (W2)
     gemm_int8_kernel<true><<<grid, 256, 0, stream>>>(a);
   else

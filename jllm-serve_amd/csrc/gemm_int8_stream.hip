@@ -1,0 +1,230 @@
+// out[m][n] = a_scale[m] * w_scale[n] * sum_k A[m][k] W[n][k] for up to 64 rows of 8-bit integers (decode steps), bound by reading W
+// from memory once.
+//
+// A workgroup owns `rows` weight rows (of each weight) and a range of K (gridDim.y of them), which its waves share in blocks of 128 bytes:
+// wave w takes blocks w, w + WAVES, .. Both operands of a block go straight from memory into a ring of S blocks in LDS that belongs
+// to the wave alone (8 rows of 128 bytes to an instruction, bank swizzle on the global side), so that nothing but the wave's own
+// count of loads in flight stands between a load and its use, and no barrier before the end. Every wave multiplies all the
+// activation rows by all the workgroup's weight rows over its blocks; the sums, whole numbers, meet in LDS.
+//
+// A compute unit's load pipe passes the activations, once per workgroup, as well as the weights: a workgroup should own about as
+// many weight rows as there are activation rows, or more. Where that leaves compute units without one, K is cut over
+// workgroups, and a second kernel adds the parts.
+//
+// Needs K % 16 == 0 and 16-byte aligned rows; any N, up to 64 rows.
+#include "int8_mfma.h"
+#include "int8_parts.h"
+#include "lds_ring.h"
+
+struct Stream8Args {
+  const signed char *A, *W, *W2;
+  int* partial;
+  int lda, ldw, K, rows, blocks;  // weight rows per workgroup; blocks of K per part
+  Int8Epilogue end;
+};
+
+template <int NI, int S>
+__device__ __forceinline__ void i8_wait_block(int behind) {  // `behind` (< S) blocks behind the one that has to be here
+  if (behind == S - 1) return wait_loads<(S - 1) * NI>();
+  if (S > 2 && behind == S - 2) return wait_loads<(S > 2 ? S - 2 : 0) * NI>();
+  if (S > 3 && behind == S - 3) return wait_loads<(S > 3 ? S - 3 : 0) * NI>();
+  if (S > 4 && behind == S - 4) return wait_loads<(S > 4 ? S - 4 : 0) * NI>();
+  if (S > 5 && behind == S - 5) return wait_loads<(S > 5 ? S - 5 : 0) * NI>();
+  wait_loads<0>();
+}
+
+// blocks of NI KB in a wave's ring: two workgroups share a compute unit where each still has two
+constexpr int i8_slots(int ni, int waves) {
+  const int shared = 79 / (waves * ni), fit = shared >= 2 ? shared : 159 / (waves * ni);
+  return fit > 6 ? 6 : fit;
+}
+
+// NW: loads of 8 weight rows per block (of each weight), NA: of 8 activation rows
+template <int NW, int NA, bool GATED, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Args p) {
+  constexpr int CT = (NW + 1) / 2, MT = (NA + 1) / 2, MATS = GATED ? 2 : 1;  // tiles of 16 weight rows (of each weight), of 16 activation rows
+  constexpr int NWT = MATS * NW, NI = NWT + NA;                             // loads of a block
+  constexpr int S = i8_slots(NI, WAVES);
+  static_assert(S >= 2 && (S - 1) * NI < 63, "the counter of loads in flight");
+  static_assert(WAVES * MATS * CT * MT <= WAVES * S * NI, "the sums fit the rings");
+  extern __shared__ __align__(1024) unsigned char smem[];  // [WAVES][S][NI KB]; afterwards the waves' sums
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int col = lane & 15, g = lane >> 4, M = p.end.M, N = p.end.N;
+  const int n0 = blockIdx.x * p.rows;
+  const int first = blockIdx.y * p.blocks, nblk = min((p.K + 127) / 128 - first, p.blocks);
+  const int tail = p.K & 127;  // bytes of the last block of K, where it is not whole
+  // ---- the loads of a block: a scalar base that advances with the block and a byte offset per lane that never changes
+  uint32_t goff[NI];
+  const int lrow = lane >> 3, lslot = lane & 7;
+#pragma unroll
+  for (int c = 0; c < NI; ++c) {
+    const bool of_w = c < NWT;
+    const int r = (of_w ? c % NW : c - NWT) * 8 + lrow;
+    const uint32_t at = of_w ? (uint32_t)(min(n0 + min(r, p.rows - 1), N - 1) - n0) * (uint32_t)p.ldw : (uint32_t)min(r, M - 1) * (uint32_t)p.lda;
+    goff[c] = at + (uint32_t)((lslot ^ ring_swz(r)) * 16);
+  }
+  const unsigned char* wbase = (const unsigned char*)p.W + (size_t)n0 * p.ldw;
+  const unsigned char* ubase = GATED ? (const unsigned char*)p.W2 + (size_t)n0 * p.ldw : nullptr;
+  const unsigned char* ring = smem + (size_t)wave * S * NI * 1024;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)ring;
+  const int total = wave < nblk ? (nblk - wave + WAVES - 1) / WAVES : 0;
+  auto issue = [&](int i, int slot) {
+    const int b = first + wave + i * WAVES;
+    const size_t kbytes = (size_t)b * 128;
+    const bool cut = tail != 0 && (b + 1) * 128 > p.K;
+#pragma unroll
+    for (int c = 0; c < NI; ++c) {
+      const unsigned char* base = (c >= NWT ? (const unsigned char*)p.A : GATED && c >= NW ? ubase : wbase) + kbytes;
+      const uint32_t to = lds0 + (uint32_t)(slot * NI + c) * 1024u;
+      if (cut) {  // pieces that are not there are zeros, of both operands
+        const int r = (c < NWT ? c % NW : c - NWT) * 8 + lrow;
+        load_to_lds_16((lslot ^ ring_swz(r)) * 16 < tail ? (const void*)(base + goff[c]) : (const void*)&int8_zeros, to);
+      } else {
+        load_to_lds_16(base, goff[c], to);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+    if (i < total) issue(i, i);
+  // ---- fragments: lane l reads row l % 16, 16 of k at (l / 16) * 16 + 64 j: piece l / 16 + 4 j. Rows that no load fetched (of an odd
+  // number of eights) are the last fetched eight again.
+  intx4 acc[MATS][CT][MT];
+#pragma unroll
+  for (int u = 0; u < MATS; ++u)
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[u][t][m] = intx4{0, 0, 0, 0};
+  auto place = [&](int loads, int t) {  // of a lane's fragment of tile t among `loads` eights
+    const int r = t * 16 + (loads - 2 * t == 1 ? col & 7 : col);
+    return r * 128 + ((g ^ ring_swz(r)) << 4);
+  };
+  int slot = 0;
+  for (int i = 0; i < total; ++i) {
+    i8_wait_block<NI, S>(min(S - 1, total - 1 - i));
+    const unsigned char* blk = ring + slot * NI * 1024;
+    u32x4 a[MT][2], w[MATS][CT][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {  // (piece + 4: bit 6 of the address)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) a[m][j] = *(const u32x4*)(blk + NWT * 1024 + (place(NA, m) ^ (j * 64)));
+#pragma unroll
+      for (int u = 0; u < MATS; ++u)
+#pragma unroll
+        for (int t = 0; t < CT; ++t) w[u][t][j] = *(const u32x4*)(blk + u * NW * 1024 + (place(NW, t) ^ (j * 64)));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot's last reads, before it is filled again
+    __builtin_amdgcn_sched_barrier(0);
+    if (i + S < total) issue(i + S, slot);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int u = 0; u < MATS; ++u)
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[u][t][m] = mfma16_i8(w[u][t][j], a[m][j], acc[u][t][m]);
+    if (++slot == S) slot = 0;
+  }
+  // ---- the waves' sums meet in LDS; then a thread has items of four columns of a row
+  __syncthreads();  // every wave is done with its ring
+  intx4(*red)[MATS][CT][MT][64] = (intx4(*)[MATS][CT][MT][64])smem;
+#pragma unroll
+  for (int u = 0; u < MATS; ++u)
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) red[wave][u][t][m][lane] = acc[u][t][m];
+  __syncthreads();
+  const bool vec = (p.end.ldo & 3) == 0 && ((uintptr_t)p.end.out & 15) == 0 && (p.rows & 3) == 0;
+  for (int item = threadIdx.x; item < CT * MT * 64; item += WAVES * 64) {
+    const int t = item / (MT * 64), mt = item / 64 % MT;
+    const int m = mt * 16 + (item & 15), in = t * 16 + (item >> 4 & 3) * 4, n = n0 + in;
+    const int there = min(4, min(N - n, p.rows - in));
+    if (m >= M || there <= 0) continue;
+    intx4 sum[MATS];
+#pragma unroll
+    for (int u = 0; u < MATS; ++u) {
+      sum[u] = intx4{0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) sum[u] += red[w][u][t][mt][item & 63];
+    }
+    if (gridDim.y > 1) {
+#pragma unroll
+      for (int u = 0; u < MATS; ++u)
+        int8_part_store(p.partial + ((size_t)blockIdx.y * MATS + u) * M * N, m, n, there, N, sum[u]);
+    } else {
+      const float sa = p.end.scales.a[m];
+      floatx4 y{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (c >= there) continue;
+        const float z = ((float)sum[0][c] * sa) * p.end.scales.w[n + c] + int8_bias(p.end, n + c);
+        y[c] = GATED ? gated<true>(z, ((float)sum[MATS - 1][c] * sa) * p.end.scales.w2[n + c], p.end.gate) : z;
+      }
+      int8_store4(p.end, m, n, there, vec, y);
+    }
+  }
+}
+
+template <int NW, int NA, bool GATED>
+static int launch_stream8(const Stream8Args& a, dim3 grid, hipStream_t stream) {
+  // four waves where their rings hold two blocks each, else two
+  constexpr int NI = (GATED ? 2 : 1) * NW + NA, WAVES = i8_slots(NI, 4) >= 2 ? 4 : 2, S = i8_slots(NI, WAVES);
+  constexpr size_t smem = (size_t)S * WAVES * NI * 1024;
+  if (hipFuncSetAttribute((const void*)gemm_int8_stream_kernel<NW, NA, GATED, WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
+    JLLM_FAIL("gemm_int8_stream: cannot reserve %zu bytes of LDS", smem);
+  gemm_int8_stream_kernel<NW, NA, GATED, WAVES><<<grid, WAVES * 64, smem, stream>>>(a);
+  return 0;
+}
+
+template <int NA, bool GATED>
+static int launch_stream8_rows(const Stream8Args& a, dim3 grid, hipStream_t stream) {
+  const int eights = (a.rows + 7) / 8;
+#define I8_EIGHTS(NW) if (eights <= NW) return launch_stream8<NW, NA, GATED>(a, grid, stream)
+  I8_EIGHTS(1); I8_EIGHTS(2); I8_EIGHTS(3); I8_EIGHTS(4); I8_EIGHTS(6); I8_EIGHTS(8); I8_EIGHTS(9); I8_EIGHTS(10); I8_EIGHTS(12);
+#undef I8_EIGHTS
+  return 1;
+}
+
+template <bool GATED>
+static int launch_stream8_batch(const Stream8Args& a, dim3 grid, hipStream_t stream) {
+  const int M = a.end.M;
+  if (M <= 8) return launch_stream8_rows<1, GATED>(a, grid, stream);
+  if (M <= 16) return launch_stream8_rows<2, GATED>(a, grid, stream);
+  if (M <= 32) return launch_stream8_rows<4, GATED>(a, grid, stream);
+  if (M <= 48) return launch_stream8_rows<6, GATED>(a, grid, stream);
+  return launch_stream8_rows<8, GATED>(a, grid, stream);
+}
+
+// `rows`: weight rows of each weight that a workgroup owns, up to 96.
+// `parts` > 1 cuts K; `partial` then holds parts * (1 or, gated, 2) * M * N ints. Returns 0 when it ran, 1 when the shape is not one it takes,
+// -1 on errors.
+extern "C" int jllm_gemm_int8_stream(const void* A, int lda, const float* a_scale, const void* W, int ldw, const float* w_scale, const void* W2, int ldw2,
+                                     const float* w2_scale, const void* bias, int bias_dtype, void* out, int out_dtype, int ldo, int M, int N, int K,
+                                     int epilogue, float gate_limit, int rows, int parts, int* partial, hipStream_t stream) {
+  if (M <= 0 || N <= 0) return 0;
+  if (M > 64 || K <= 0 || K > I8_MOST_K || (K & 15) || (lda & 15) || (ldw & 15) || (W2 && ldw2 != ldw)) return 1;
+  if (((uintptr_t)A & 15) || ((uintptr_t)W & 15) || ((uintptr_t)W2 & 15)) return 1;
+  JLLM_TAKE_GATE("gemm_int8_stream", epilogue, gate_limit, gs);
+  if (epilogue < 0 || epilogue > 2 || (epilogue == 2) != (W2 != nullptr)) JLLM_FAIL("gemm_int8_stream: epilogue %d", epilogue);
+  if (epilogue == 1 && out_dtype != JLLM_F32) JLLM_FAIL("gemm_int8_stream: the accumulate epilogue adds into fp32");
+  if (lda < 0 || ldw < 0 || ldo < N) JLLM_FAIL("gemm_int8_stream: rows %d, %d and %d apart", lda, ldw, ldo);
+  if (rows < 1 || rows > 96) JLLM_FAIL("gemm_int8_stream: %d weight rows per workgroup (1 to 96)", rows);
+  // a lane's place in an operand is a 32-bit byte offset from the workgroup's first row
+  if ((unsigned)lda >= (1u << 25) || (unsigned)ldw >= (1u << 25)) return 1;
+  const int blocks = (K + 127) / 128;
+  parts = parts < 1 ? 1 : parts > blocks ? blocks : parts;
+  const int each = (blocks + parts - 1) / parts;
+  parts = (blocks + each - 1) / each;  // those that have any block
+  if (parts > 65535) return 1;
+  if (parts > 1 && (!partial || ((uintptr_t)partial & 15))) JLLM_FAIL("gemm_int8_stream: %d parts of K need a buffer for their sums", parts);
+  const Stream8Args a{(const signed char*)A, (const signed char*)W, (const signed char*)W2, partial, lda, ldw, K, rows, each,
+                      {{a_scale, w_scale, w2_scale}, bias, out, bias_dtype, out_dtype, ldo, M, N, epilogue, gs}};
+  const dim3 grid((N + rows - 1) / rows, parts);
+  const int rc = W2 ? launch_stream8_batch<true>(a, grid, stream) : launch_stream8_batch<false>(a, grid, stream);
+  if (rc != 0) return rc;
+  JLLM_CHECK_LAUNCH("gemm_int8_stream");
+  return parts > 1 ? int8_add_parts(partial, parts, a.end, W2 != nullptr, stream) : 0;
+}

@@ -6,10 +6,9 @@
 //
 // The sums are exact (up to 131,071 inputs, where 128^2 K stays below 2^31), so an output does not depend on the tile, the cut of
 // K or the order in which parts are added. It is (float(sum) * a_scale[m]) * w_scale[n], and from there on what the other
-// products' epilogue makes of a sum (gemm_epilogue.h).
+// products make of a sum.
 #pragma once
 #include "common.h"
-#include "gemm_epilogue.h"
 #include "mfma.h"
 
 typedef int intx4 __attribute__((ext_vector_type(4)));
@@ -20,29 +19,101 @@ __device__ __forceinline__ intx4 mfma16_i8(u32x4 a, u32x4 b, intx4 c) {
 
 #define I8_MOST_K 131071
 
+// what loads of pieces behind the end of K fetch instead
+__device__ const uint4 int8_zeros{0u, 0u, 0u, 0u};
+
 struct Int8Scales {
   const float *a, *w, *w2;  // per row of A, per row of W (and of the second weight)
 };
 
-// A wave's accumulators as tile_epilogue takes them: runs [.][j] of the first weight's outputs and, gated, [.][j + CN / 2] of the second's
-template <bool GATED, int RM, int CN, int TBM, int TBN>
-__device__ __forceinline__ void int8_epilogue(intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Scales& sc, const void* bias,
-                                              int bias_dtype, void* out, int out_dtype, int ldo, int M, int N, int epilogue, GateSpec gs) {
+// What is done with a sum: the first weight's (with a bias and, gated, the second's), as the product's output
+struct Int8Epilogue {
+  Int8Scales scales;
+  const void* bias;
+  void* out;
+  int bias_dtype, out_dtype, ldo, M, N, epilogue;
+  GateSpec gate;
+};
+
+__device__ __forceinline__ float int8_bias(const Int8Epilogue& p, int n) {
+  return !p.bias ? 0.f : p.bias_dtype == JLLM_BF16 ? ldf((const bf16_t*)p.bias, n) : ldf((const float*)p.bias, n);
+}
+
+// Four neighbouring outputs of row m from column n on, of which `there` exist; `vec`: the row's places from n on are 16-byte aligned (8 in bf16)
+__device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n, int there, bool vec, floatx4 v) {
+  const size_t o = (size_t)m * p.ldo + n;
+  if (there == 4 && vec) {
+    if (p.epilogue == 1) {
+      floatx4* to = (floatx4*)((float*)p.out + o);
+      *to = *to + v;
+    } else if (p.out_dtype == JLLM_BF16) {
+      *(u32x2*)((bf16_t*)p.out + o) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    } else {
+      *(floatx4*)((float*)p.out + o) = v;
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (c >= there) continue;
+    if (p.epilogue == 1)
+      ((float*)p.out)[o + c] += v[c];
+    else if (p.out_dtype == JLLM_BF16)
+      stf((bf16_t*)p.out, o + c, v[c]);
+    else
+      stf((float*)p.out, o + c, v[c]);
+  }
+}
+
+// A wave's accumulators, CN runs of four columns for each of its RM blocks of 16 rows (gated: [.][j] and [.][j + CN / 2] are the two weights' of the
+// same outputs), row block by row block, so that hardly more than the sums themselves is in registers.
+template <bool GATED, int RM, int CN>
+__device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
   constexpr int NI = GATED ? CN / 2 : CN;
-  const int row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * NI * 16 + lane / 16 * 4;
-  float sa[RM], sw[CN][4];
+  const int group = lane / 16, row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * NI * 16 + group * 4;
+  float sw[NI][4], su[NI][4], bv[NI][4];
 #pragma unroll
-  for (int i = 0; i < RM; ++i) sa[i] = sc.a[min(row0 + i * 16, M - 1)];
+  for (int j = 0; j < NI; ++j)
 #pragma unroll
-  for (int j = 0; j < CN; ++j)
+    for (int c = 0; c < 4; ++c) {
+      const int n = min(col0 + j * 16 + c, p.N - 1);
+      sw[j][c] = p.scales.w[n];
+      su[j][c] = GATED ? p.scales.w2[n] : 0.f;
+      bv[j][c] = int8_bias(p, n);
+    }
+  const bool vec = (p.ldo & 3) == 0 && ((uintptr_t)p.out & 15) == 0;
+  const bool whole = n0 + (wn + 1) * NI * 16 <= p.N;  // the wave's columns are all there
+  // in bf16 two neighbouring runs exchange halves between lanes first, so that a lane stores eight columns
+  const bool eights = NI % 2 == 0 && whole && vec && (p.ldo & 7) == 0 && p.epilogue != 1 && p.out_dtype == JLLM_BF16;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) sw[j][c] = (GATED && j >= NI ? sc.w2 : sc.w)[min(col0 + j % NI * 16 + c, N - 1)];
-  floatx4 v[RM][CN];
+  for (int i = 0; i < RM; ++i) {
+    const int m = row0 + i * 16;
+    const float sa = p.scales.a[min(m, p.M - 1)];
+    auto outputs = [&](int j) {
+      floatx4 v;
 #pragma unroll
-  for (int i = 0; i < RM; ++i)
+      for (int c = 0; c < 4; ++c) {
+        const float z = ((float)acc[i][j][c] * sa) * sw[j][c] + bv[j][c];
+        v[c] = GATED ? gated<true>(z, ((float)acc[i][GATED ? NI + j : 0][c] * sa) * su[j][c], p.gate) : z;
+      }
+      return v;
+    };
+    if (m >= p.M) continue;
+    if (eights) {
 #pragma unroll
-    for (int j = 0; j < CN; ++j)
+      for (int j = 0; j < NI / 2 * 2; j += 2) {
+        const floatx4 v = outputs(j), w = outputs(j + 1);
+        const u32x2 lo = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])}, hi = {pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3])};
+        const auto a = __builtin_amdgcn_permlane16_swap(lo.x, hi.x, false, false);
+        const auto b = __builtin_amdgcn_permlane16_swap(lo.y, hi.y, false, false);
+        *(u32x4*)((bf16_t*)p.out + (size_t)m * p.ldo + col0 + j * 16 - group * 4 + (group & 1) * 16 + (group >> 1) * 8) = u32x4{a[0], b[0], a[1], b[1]};
+      }
+    } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v[i][j][c] = ((float)acc[i][j][c] * sa[i]) * sw[j][c];
-  tile_epilogue<GATED, RM, CN, TBM, TBN>(v, lane, wm, wn, m0, n0, bias, bias_dtype, out, out_dtype, ldo, M, N, epilogue, gs, nullptr, 0, 1);
+      for (int j = 0; j < NI; ++j) {
+        const int n = col0 + j * 16;
+        if (n < p.N) int8_store4(p, m, n, min(4, p.N - n), vec, outputs(j));
+      }
+    }
+  }
 }

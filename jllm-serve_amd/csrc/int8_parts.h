@@ -1,0 +1,77 @@
+// Products of 8-bit integers whose K is cut over workgroups: the parts' whole-number sums in memory and the kernel that adds them.
+#pragma once
+#include "int8_mfma.h"
+
+// what the tiled kernels take
+struct Int8Args {
+  const signed char *A, *W, *W2;
+  int* partial;  // [part][M][N]
+  int lda, ldw, K;
+  Int8Epilogue end;
+};
+
+// four neighbouring sums of row m from column n on, of which `there` exist
+__device__ __forceinline__ void int8_part_store(int* __restrict__ part, int m, int n, int there, int N, intx4 v) {
+  int* to = part + (size_t)m * N + n;
+  if (there >= 4 && ((N | n) & 3) == 0) {
+    *(intx4*)to = v;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (c < there) to[c] = v[c];
+  }
+}
+
+// A wave's sums as its part of a cut K
+template <int RM, int CN>
+__device__ __forceinline__ void int8_partial(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, int* part, int M, int N) {
+  const int row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * CN * 16 + lane / 16 * 4;
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < CN; ++j)
+      if (row0 + i * 16 < M) int8_part_store(part, row0 + i * 16, col0 + j * 16, N - col0 - j * 16, N, acc[i][j]);
+}
+
+// The parts' sums ([part][weight][M][N]), V neighbouring outputs per thread (4, or 1 where N is no multiple of four): exact, so in any order
+template <int V, bool GATED>
+__global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__ partial, int parts, Int8Epilogue p) {
+  constexpr int MATS = GATED ? 2 : 1;
+  const size_t all = (size_t)p.M * p.N, i = ((size_t)blockIdx.x * 256 + threadIdx.x) * V;
+  if (i >= all) return;
+  const int m = (int)(i / p.N), n = (int)(i - (size_t)m * p.N);
+  int sum[MATS][V] = {};
+#pragma unroll 4
+  for (int z = 0; z < parts; ++z)
+#pragma unroll
+    for (int u = 0; u < MATS; ++u) {
+      int s[V];
+      __builtin_memcpy(s, (const int*)__builtin_assume_aligned(partial + ((size_t)z * MATS + u) * all + i, 4 * V), sizeof(s));
+#pragma unroll
+      for (int c = 0; c < V; ++c) sum[u][c] += s[c];
+    }
+  const float sa = p.scales.a[m];
+  floatx4 y{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const float z = ((float)sum[0][c] * sa) * p.scales.w[n + c] + int8_bias(p, n + c);
+    y[c] = GATED ? gated<true>(z, ((float)sum[MATS - 1][c] * sa) * p.scales.w2[n + c], p.gate) : z;
+  }
+  int8_store4(p, m, n, V, V == 4 && (p.ldo & 3) == 0 && ((uintptr_t)p.out & 15) == 0, y);
+}
+
+static inline int int8_add_parts(const int* partial, int parts, const Int8Epilogue& end, bool gated, hipStream_t stream) {
+  const int v = end.N % 4 == 0 ? 4 : 1;
+  const size_t groups = ((size_t)end.M * end.N / v + 255) / 256;
+  if (groups > 0x7fffffffull) JLLM_FAIL("gemm_int8: %d x %d outputs are more than a grid takes", end.M, end.N);
+  const unsigned n = (unsigned)groups;
+  if (gated) {
+    if (v == 4) int8_parts_kernel<4, true><<<n, 256, 0, stream>>>(partial, parts, end);
+    else int8_parts_kernel<1, true><<<n, 256, 0, stream>>>(partial, parts, end);
+  } else {
+    if (v == 4) int8_parts_kernel<4, false><<<n, 256, 0, stream>>>(partial, parts, end);
+    else int8_parts_kernel<1, false><<<n, 256, 0, stream>>>(partial, parts, end);
+  }
+  JLLM_CHECK_LAUNCH("gemm_int8: the sum of the parts");
+  return 0;
+}

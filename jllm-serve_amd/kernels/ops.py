@@ -11,6 +11,7 @@ import bisect
 import contextlib
 import ctypes
 import functools
+import math
 import struct
 import threading
 from typing import Optional, Tuple
@@ -128,6 +129,9 @@ def _declare(lib) -> None:
 
 
 _OPTIONAL_SIGS = {
+    "jllm_gemm_int8_stream": [_P, _I, _P, _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P],
+    "jllm_gemm_int8_tiled": [_P, _I, _P, _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P],
+    "jllm_gemm_int8_large": [_P, _I, _P, _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P],
     "jllm_gemm_skinny_bf16": [_P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P],
     "jllm_gemm_skinny_norm_bf16": [_P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _I, _P, _I, _P, _I, _F, _P],
     "jllm_gemm_mfma_bf16": [_P, _I, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _I, _F, _P, _I, _P],
@@ -817,10 +821,108 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
     if M == 0 or N == 0:
         return out
     epilogue = int(epilogue) | (int(gate) << 8)  # the kernels take it apart again and refuse what they do not have
-    _call("jllm_gemm_int8", _ptr(a.q), _distance(a.q), _ptr(a.scale), _ptr(w.q), _distance(w.q), _ptr(w.scale), _ptr(w2.q) if w2 else None,
-          _distance(w2.q) if w2 else 0, _ptr(w2.scale) if w2 else None, _ptr(bias), bias_code, _ptr(out), out_code, _distance(out), M, N, K,
-          int(epilogue), float(gate_limit), _stream())
+    head = (_ptr(a.q), _distance(a.q), _ptr(a.scale), _ptr(w.q), _distance(w.q), _ptr(w.scale), _ptr(w2.q) if w2 is not None else None,
+            _distance(w2.q) if w2 is not None else 0, _ptr(w2.scale) if w2 is not None else None, _ptr(bias), bias_code, _ptr(out), out_code,
+            _distance(out), M, N, K, epilogue, float(gate_limit))
+    for kernel, size, parts in _int8_plans(M, N, K, w2 is not None) if K % 16 == 0 else ():
+        sums = torch.empty((parts * M * N * (2 if w2 is not None else 1),), dtype=torch.int32, device=out.device) if parts > 1 else None
+        if _try(kernel, *head, size, parts, _ptr(sums), _stream()):
+            return out
+    _count("general", "jllm_gemm_int8")
+    _call("jllm_gemm_int8", *head, _stream())
     return out
+
+
+INT8_STREAM_MOST_ROWS = 64  # of activations that the weight-streaming kernel takes
+INT8_STREAM_LOADS = (1, 2, 4, 6, 8)  # its loads of eight activation rows ...
+INT8_STREAM_WEIGHT_LOADS = (1, 2, 3, 4, 6, 8, 9, 10, 12)  # ... and of eight rows of each weight
+INT8_STREAM_WEIGHTS = (8, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64, 72, 80, 96)  # rows of each weight to a workgroup
+INT8_CUTS = (1, 2, 3, 4, 6, 8)
+INT8_CUT_MIN_K = 512          # of a part
+INT8_CUT_MOST_GROUPS = 640    # workgroups of a cut product: more of them gain nothing
+INT8_STREAM_CUT_US = (1.54, 3.0e-6)  # a cut of K: the second launch, and per sum of a part, of which there are few ...
+INT8_TILE_CUT_US = (2.62, 1.12e-6)   # ... and many
+
+
+def _int8_stream_us(M: int, N: int, K: int, weights: int, rows: int, parts: int) -> float:
+    """Estimated time of a product of up to 64 rows in workgroups of ``rows`` weight rows (of each of ``weights`` weights) and K in ``parts``:
+    the bytes that the busiest compute unit's load pipe passes, 44.5 a nanosecond (an activation row counts for 0.59: the workgroups
+    of a compute unit ask for the same ones), against the weights' way from memory, and rounds of workgroups. Fitted to 2,800 times
+    of 15 products (0.6B to 32B shapes and three others) at 1 to 64 rows, inside a graph over as many weights as do not fit the caches: 10 % off on
+    average, and the cheapest by the estimate 1.4 % behind the best choice on average, 20 % at worst."""
+    cus = compute_units()
+    loads = weights * next(n for n in INT8_STREAM_WEIGHT_LOADS if 8 * n >= rows) + M // 8
+    shared = 79 // (4 * loads) >= 2  # two workgroups fit a compute unit
+    blocks = -(-K // 128)
+    each = -(-blocks // parts)
+    groups = -(-N // rows) * -(-blocks // each)
+    pipe = -(-groups // cus) * (weights * -(-rows // 8) * 8 + 0.59 * M) * each * 128 / 44.5e3
+    memory = weights * N * K / 5.73e6
+    us = 3.2 + (pipe ** 2.25 + memory ** 2.25) ** (1 / 2.25) + 1.6 * (-(-groups // (2 * cus if shared else cus)) - 1)
+    return us + (INT8_STREAM_CUT_US[0] + INT8_STREAM_CUT_US[1] * parts * M * N * weights if parts > 1 else 0.0)
+
+
+# Estimated times of the tiles, in microseconds, by rows * 1000 + columns: (fixed, a stage of 128 of K with few compute units at work, what
+# it takes more with all, a round of workgroups beside its stages), and for the two of which a compute unit holds two the second and third
+# again where all hold one and some hold two. The first three go through csrc/gemm_int8_tiled.hip, the others through gemm_int8_large.hip.
+INT8_TILE_US = {64064: (3.44, 0.198, 0.028, 1.53, 0.348, 0.072), 64128: (4.37, 0.316, 0.076, 1.30, 0.516, 0.152), 128128: (3.12, 0.370, 0.171, 4.12),
+                128256: (3.85, 0.552, 0.346, 3.80), 256128: (4.54, 0.512, 0.328, 3.56), 192256: (4.49, 0.774, 0.324, 5.33), 256256: (5.07, 0.966, 0.396, 6.46)}
+INT8_LARGE_FROM = 128256
+INT8_TILE_BYTES_PER_US = 4.54e6
+
+
+def _int8_tile_us(tile: int, M: int, N: int, K: int, weights: int, parts: int) -> float:
+    """The product in tiles of one kind with K in ``parts``: rounds of workgroups, one or two to a compute unit, against the weights' way from
+    memory. Fitted to 3,500 times of 14 products at 80 to 4,096 rows, taken as for `_int8_stream_us`: 8 % off on average, the cheapest by
+    the estimate 0.5 % behind the best choice on average, 10 % at worst (without the tiles of 64 x 64 9 %, without either of the others 1 to 2 %
+    on average)."""
+    cus = compute_units()
+    rows, columns = divmod(tile, 1000)
+    fixed, lone, more, round_us, *pair = INT8_TILE_US[tile]
+    stages = -(--(-K // 128) // parts)
+    groups = -(-N // (columns // weights)) * -(-M // rows) * parts
+    full, rest = divmod(groups, 2 * cus if pair else cus)
+    us = full * (stages * (sum(pair) if pair else lone + more) + round_us)
+    if rest > cus:
+        us += stages * (pair[0] + pair[1] * (rest - cus) / cus) + round_us
+    elif rest:
+        us += stages * (lone + more * rest / cus) + round_us
+    us = fixed + math.hypot(us, weights * N * K / INT8_TILE_BYTES_PER_US)
+    return us + (INT8_TILE_CUT_US[0] + INT8_TILE_CUT_US[1] * parts * M * N if parts > 1 else 0.0)
+
+
+@functools.lru_cache(maxsize=8192)
+def _int8_choices(units: int, N: int, K: int, gated: bool):
+    """`_int8_plans` for ``units`` rows: 8 times one of INT8_STREAM_LOADS, or a multiple of 64 above."""
+    weights = 2 if gated else 1
+    stages = -(-K // 128)
+
+    def cuts(groups, most_cuts=INT8_CUTS):
+        for parts in most_cuts:
+            # (every part has stages of its own)
+            if parts == 1 or (K // parts >= INT8_CUT_MIN_K and groups * parts <= INT8_CUT_MOST_GROUPS and stages > -(-stages // parts) * (parts - 1)):
+                yield parts
+
+    if units <= INT8_STREAM_MOST_ROWS:
+        best = min((_int8_stream_us(units, N, K, weights, rows, parts), rows, parts) for rows in INT8_STREAM_WEIGHTS
+                   for parts in cuts(-(-N // rows), INT8_CUTS if rows >= 16 else (1,)))
+        return (("jllm_gemm_int8_stream", best[1], best[2]),)
+    found = []
+    for large in (False, True):
+        if large and K <= 128:
+            continue
+        found.append(min((_int8_tile_us(tile, units, N, K, weights, parts), tile, parts) for tile in INT8_TILE_US if (tile >= INT8_LARGE_FROM) == large
+                         for parts in cuts(-(-N // (tile % 1000 // weights)) * -(-units // (tile // 1000)), (1,) if gated else INT8_CUTS)))
+    found.sort()
+    # (the large tiles decline operands of 4 GB: then the others' best)
+    return tuple(("jllm_gemm_int8_large" if tile >= INT8_LARGE_FROM else "jllm_gemm_int8_tiled", tile, parts) for _, tile, parts in found)
+
+
+def _int8_plans(M: int, N: int, K: int, gated: bool):
+    """(entry point, its tile or weight rows, parts of K) of the fast kernels for a product, the cheapest by the estimates first."""
+    if M <= INT8_STREAM_MOST_ROWS:
+        return _int8_choices(8 * next(n for n in INT8_STREAM_LOADS if 8 * n >= M), N, K, gated)
+    return _int8_choices(-(-M // 64) * 64, N, K, gated)
 
 
 MAX_HEAD_DIM = 512     # what the general attention kernel takes (csrc/attention_generic.hip); the fast ones take less
