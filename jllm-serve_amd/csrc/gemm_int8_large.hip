@@ -36,8 +36,7 @@ static int launch_int8_large(const Int8Args& a, int parts, hipStream_t stream) {
   const dim3 grid((a.end.N + cols - 1) / cols, (a.end.M + TBM - 1) / TBM, parts);
   if (grid.y > 65535 || (unsigned long long)grid.x * grid.y > 0x7fffffffull) return 1;
   constexpr size_t smem = PingpongRing<FM, WGM>::BYTES;
-  const void* kernel = a.W2 ? (const void*)gemm_int8_large_kernel<true, FM, WGM> : (const void*)gemm_int8_large_kernel<false, FM, WGM>;
-  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
+  if (!(a.W2 ? int8_allow_lds<gemm_int8_large_kernel<true, FM, WGM>>((int)smem) : int8_allow_lds<gemm_int8_large_kernel<false, FM, WGM>>((int)smem)))
     JLLM_FAIL("gemm_int8_large: cannot reserve %zu bytes of LDS", smem);
   if (a.W2)
     gemm_int8_large_kernel<true, FM, WGM><<<grid, PP_WAVES * 64, smem, stream>>>(a);

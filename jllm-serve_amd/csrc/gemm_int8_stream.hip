@@ -173,7 +173,7 @@ static int launch_stream8(const Stream8Args& a, dim3 grid, hipStream_t stream) {
   // four waves where their rings hold two blocks each, else two
   constexpr int NI = (GATED ? 2 : 1) * NW + NA, WAVES = i8_slots(NI, 4) >= 2 ? 4 : 2, S = i8_slots(NI, WAVES);
   constexpr size_t smem = (size_t)S * WAVES * NI * 1024;
-  if (hipFuncSetAttribute((const void*)gemm_int8_stream_kernel<NW, NA, GATED, WAVES>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != hipSuccess)
+  if (!int8_allow_lds<gemm_int8_stream_kernel<NW, NA, GATED, WAVES>>((int)smem))
     JLLM_FAIL("gemm_int8_stream: cannot reserve %zu bytes of LDS", smem);
   gemm_int8_stream_kernel<NW, NA, GATED, WAVES><<<grid, WAVES * 64, smem, stream>>>(a);
   return 0;

@@ -164,7 +164,7 @@ static int launch_int8_tiled(const Int8Args& a, int parts, hipStream_t stream) {
   static_assert(LDS <= 160 * 1024, "the ring fits");
   const dim3 grid((a.end.N + COLS - 1) / COLS, (a.end.M + TBM - 1) / TBM, parts);
   if (grid.y > 65535 || (unsigned long long)grid.x * grid.y > 0x7fffffffull) return 1;
-  if (hipFuncSetAttribute((const void*)gemm_int8_tiled_kernel<GATED, RM, CN, WGM, WGN, NS>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+  if (!int8_allow_lds<gemm_int8_tiled_kernel<GATED, RM, CN, WGM, WGN, NS>>(LDS))
     JLLM_FAIL("gemm_int8_tiled: cannot reserve %d bytes of LDS", LDS);
   gemm_int8_tiled_kernel<GATED, RM, CN, WGM, WGN, NS><<<grid, WGM * WGN * 64, LDS, stream>>>(a);
   return 0;

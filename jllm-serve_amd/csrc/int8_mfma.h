@@ -8,6 +8,7 @@
 // K or the order in which parts are added. It is (float(sum) * a_scale[m]) * w_scale[n], and from there on what the other
 // products make of a sum.
 #pragma once
+#include <atomic>
 #include "common.h"
 #include "mfma.h"
 
@@ -116,4 +117,17 @@ __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int la
       }
     }
   }
+}
+
+// Above 64 KB a kernel's dynamic LDS has to be allowed first, on every device once
+template <auto KERNEL>
+static inline bool int8_allow_lds(int bytes) {
+  static std::atomic<unsigned long long> allowed{0};
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) return false;
+  const unsigned long long bit = device < 64 ? 1ull << device : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return true;
+  if (hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }

@@ -75,7 +75,8 @@ _SIGS = {
     "jllm_quantize_rows": [_P, _I, _I, _I, _I, _P, _I, _P, _P],
     "jllm_dequantize_rows": [_P, _I, _P, _I, _I, _P, _I, _I, _P],
     "jllm_rmsnorm_int8": [_P, _I, _P, _I, _I, _P, _I, _I, _I, _P, _I, _F, _P, _I, _P, _P],
-    "jllm_gemm_int8": [_P, _I, _P, _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _P],
+    "jllm_gemm_int8": [_P, _I, _P, _P, _I, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P],
+    "jllm_int8_lay_out": [_P, _I, _P, _I, _I, _I, _P],
     "jllm_latent_prepare": [_P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _F, _P, _P, _P, _P, _P, _I, _P, _P],
     "jllm_latent_heads_generic": [_P, _I, _I, _I, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P],
     "jllm_latent_attention_generic": [_P, _I, _P, _I, _I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P],
@@ -674,56 +675,68 @@ class Int8Rows:
 
     def tensor(self, dtype: torch.dtype) -> torch.Tensor:
         """The values that the rows stand for, rounded once to ``dtype``."""
-        _int8_rows(self, "rows")
+        n, width, distance = _int8_rows(self, "rows")
         code = _code(dtype)
         _here(self.q, self.scale)
-        n, width = self.q.shape
         out = activation_rows(n, width, dtype, self.q.device)
         if n and width:
-            _call("jllm_dequantize_rows", _ptr(self.q), _distance(self.q), _ptr(self.scale), n, width, _ptr(out), code, _distance(out), _stream())
+            _call("jllm_dequantize_rows", self.q.data_ptr(), distance, self.scale.data_ptr(), n, width, out.data_ptr(), code, _rows_of(out, "values")[2],
+                  _stream())
         return out
 
 
 INT8_MOST_INPUTS = 131071  # of a product: 128^2 times as many stay below 2^31, so every sum is exact
 
 
-def _distance(t: torch.Tensor) -> int:
-    """Entries between the rows of a 2-D tensor; a single row's stride says nothing."""
-    apart = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if apart >= 1 << 31 or t.shape[0] >= 1 << 31:
-        raise KernelError(f"the kernels take fewer than 2^31 rows, less than 2^31 entries apart; got {tuple(t.shape)}, strides {t.stride()}")
-    return apart
+# (These products take a few microseconds, and so does the host for each: what follows asks a tensor for its sizes once.)
+
+
+def _rows_of(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
+    """(rows, width, entries from one row to the next) of a 2-D tensor with contiguous rows; a single row's stride says nothing."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or strides[1] != 1:
+        raise KernelError(f"{what} must be a 2-D tensor with contiguous rows, got shape {tuple(shape)} strides {strides}")
+    n, width = shape
+    distance = strides[0] if n > 1 else width
+    if distance >= 1 << 31 or n >= 1 << 31:
+        raise KernelError(f"{what}: the kernels take fewer than 2^31 rows, less than 2^31 entries apart; got {tuple(shape)}, strides {strides}")
+    return n, width, distance
+
+
+def _own_rows_of(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
+    """The same of rows that are written: none over another."""
+    found = _rows_of(t, what)
+    if found[2] < found[1]:
+        raise KernelError(f"{what} must have rows of their own, got shape {tuple(t.shape)} strides {t.stride()}")
+    return found
 
 
 def _here(*tensors) -> None:
     """All on the current GPU, on whose stream the launch goes."""
-    _dev(*tensors)
-    now = _raw_device()
+    now = _raw_device() if tensors[0].is_cuda else -2
     for t in tensors:
         if t is not None and t.get_device() != now:
+            _dev(*tensors)
             raise KernelError(f"the engine's kernels run on the current GPU (cuda:{now}); got a tensor on {t.device}")
 
 
-def _apart(t: torch.Tensor, what: str) -> None:
-    """Rows that are written: none over another."""
-    if _distance(t) < t.shape[1]:
-        raise KernelError(f"{what} must have rows of their own, got shape {tuple(t.shape)} strides {t.stride()}")
-
-
-def _int8_rows(rows: Int8Rows, what: str) -> None:
+def _int8_rows(rows: Int8Rows, what: str) -> Tuple[int, int, int]:
     if not isinstance(rows, Int8Rows):
         raise KernelError(f"{what} must be Int8Rows, got {type(rows).__name__}")
-    if rows.q.dtype != torch.int8:
-        raise KernelError(f"{what} must be int8, got {rows.q.dtype}")
-    _rows2d(rows.q, what)
-    if rows.scale.dtype != torch.float32 or rows.scale.dim() != 1 or rows.scale.shape[0] != rows.q.shape[0] or not rows.scale.is_contiguous():
-        raise KernelError(f"{what}: the scales must be a contiguous fp32 tensor with one entry per row ({rows.q.shape[0]}), got "
-                          f"{rows.scale.dtype} {tuple(rows.scale.shape)}")
+    q, scale = rows.q, rows.scale
+    if q.dtype != torch.int8:
+        raise KernelError(f"{what} must be int8, got {q.dtype}")
+    found = _rows_of(q, what)
+    if scale.dtype != torch.float32 or scale.shape != (found[0],) or not scale.is_contiguous():
+        raise KernelError(f"{what}: the scales must be a contiguous fp32 tensor with one entry per row ({found[0]}), got "
+                          f"{scale.dtype} {tuple(scale.shape)}")
+    return found
 
 
-def _vector(t: Optional[torch.Tensor], n: int, what: str) -> None:
-    if t is not None and (t.numel() != n or not t.is_contiguous()):
+def _vector_code(t: torch.Tensor, n: int, what: str) -> int:
+    if t.numel() != n or not t.is_contiguous():
         raise KernelError(f"{what} has {t.numel()} entries for rows of {n}")
+    return _code(t.dtype)
 
 
 def _new_int8_rows(n: int, width: int, device) -> Int8Rows:
@@ -734,15 +747,14 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """Rows of ``x`` (fp32 or bf16 [n, width], any distance apart) as 8-bit integers: scale = max |x| / 127, q = x * (127 / max |x|)
     rounded to the nearest whole number, halves to even. A row of zeros has scale 0; one with a NaN or an infinity has scale NaN
     and zeros, so that what is computed from it is NaN. For activations in front of ``gemm_int8``, and for a weight [N, K] at load."""
-    _rows2d(x, "quantize_rows input")
-    dtype = _code(x.dtype)
-    n, width = x.shape
+    n, width, distance = _rows_of(x, "quantize_rows input")
+    code = _code(x.dtype)
     if width == 0:
         raise KernelError("quantize_rows: rows without entries have no scale")
     _here(x)
     out = _new_int8_rows(n, width, x.device)
     if n:
-        _call("jllm_quantize_rows", _ptr(x), dtype, _distance(x), n, width, _ptr(out.q), _distance(out.q), _ptr(out.scale), _stream())
+        _call("jllm_quantize_rows", x.data_ptr(), code, distance, n, width, out.q.data_ptr(), width, out.scale.data_ptr(), _stream())
     return out
 
 
@@ -753,30 +765,31 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
     ``x + add``, and the sum goes to ``out`` (fp32; not given: into ``x``, the residual stream)."""
     if x.dtype != torch.float32:
         raise KernelError("rmsnorm_int8 takes fp32 rows")
-    _rows2d(x, "rmsnorm_int8 input")
-    n, width = x.shape
+    n, width, distance = _rows_of(x, "rmsnorm_int8 input")
     if width == 0:
         raise KernelError("rmsnorm_int8: rows without entries have no norm")
-    _vector(gain, width, "rmsnorm_int8 gain")
+    gain_code = _vector_code(gain, width, "rmsnorm_int8 gain")
     if add is None:
         if out is not None:
             raise KernelError("rmsnorm_int8: a place for the sum without rows to add")
+        joins = (None, F32, 0, None, 0)
+        _here(x, gain)
     else:
-        _rows2d(add, "rmsnorm_int8 rows to add")
+        _, _, add_distance = _rows_of(add, "rmsnorm_int8 rows to add")
         if add.shape != x.shape:
             raise KernelError(f"rmsnorm_int8: rows to add {tuple(add.shape)} for {tuple(x.shape)}")
-        out = x if out is None else out
-        _rows2d(out, "rmsnorm_int8 sum")
+        add_code = _code(add.dtype)
+        if out is None:
+            out = x
+        _, _, out_distance = _own_rows_of(out, "rmsnorm_int8 sum")
         if out.dtype != torch.float32 or out.shape != x.shape:
             raise KernelError(f"rmsnorm_int8: the sum goes to an fp32 tensor of x's shape, got {out.dtype} {tuple(out.shape)}")
-        _apart(out, "rmsnorm_int8 sum")
-    gain_code, add_code = _code(gain.dtype), _code(add.dtype) if add is not None else F32
-    _here(x, gain, add, out)
+        joins = (add.data_ptr(), add_code, add_distance, out.data_ptr(), out_distance)
+        _here(x, gain, add, out)
     rows = _new_int8_rows(n, width, x.device)
     if n:
-        _call("jllm_rmsnorm_int8", _ptr(x), _distance(x), _ptr(add), add_code, _distance(add) if add is not None else 0, _ptr(out),
-              _distance(out) if out is not None else 0, n, width, _ptr(gain), gain_code, float(eps), _ptr(rows.q), _distance(rows.q), _ptr(rows.scale),
-              _stream())
+        _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, rows.q.data_ptr(), width,
+              rows.scale.data_ptr(), _stream())
     return rows
 
 
@@ -786,51 +799,83 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
     """out[m, n] = a.scale[m] * w.scale[n] * sum_k a.q[m, k] * w.q[n, k] (+ bias[n]): a product of 8-bit rows with a weight's output
     channels. The sums are whole numbers and exact (up to 131,071 inputs), so a row has the same bits whatever rows stand
     beside it. Epilogues and gate functions as in ``gemm``: EPI_STORE writes ``out_dtype`` (bf16 where nothing is said), EPI_ADD adds into
-    the fp32 ``out``, EPI_GATED writes gate(a w + bias, a w2)."""
-    _int8_rows(a, "gemm_int8 input")
-    _int8_rows(w, "gemm_int8 weight")
-    M, K = a.q.shape
-    N = w.q.shape[0]
-    if w.q.shape[1] != K:
-        raise KernelError(f"gemm_int8: input rows have {K} entries, weight rows {w.q.shape[1]}")
+    the fp32 ``out``, EPI_GATED writes gate(a w + bias, a w2). Rows of any number of entries at any alignment are taken; the fast kernels
+    ask for multiples of 16 that begin on 16 bytes."""
+    M, K, lda = _int8_rows(a, "gemm_int8 input")
+    N, inputs, ldw = _int8_rows(w, "gemm_int8 weight")
+    if inputs != K:
+        raise KernelError(f"gemm_int8: input rows have {K} entries, weight rows {inputs}")
     if not 0 < K <= INT8_MOST_INPUTS:
         raise KernelError(f"gemm_int8: rows of {K} entries (1 to {INT8_MOST_INPUTS}: beyond, the sums could leave 32 bits)")
     if epilogue not in (EPI_STORE, EPI_ADD, EPI_GATED) or (epilogue == EPI_GATED) != (w2 is not None):
         raise KernelError("gemm_int8: the gated epilogue takes exactly two weights")
-    if w2 is not None:
-        _int8_rows(w2, "gemm_int8 second weight")
-        if w2.q.shape != w.q.shape:
-            raise KernelError("gemm_int8: the two weights of the gated epilogue must agree in shape")
     if gate and (epilogue != EPI_GATED or not 0 < gate < (1 << 20)):
         raise KernelError(f"gemm_int8: gate function {gate} without the gated epilogue")
-    _vector(bias, N, "gemm_int8 bias")
-    bias_code = _code(bias.dtype) if bias is not None else F32
+    gated = w2 is not None
+    if gated:
+        _, _, ldw2 = _int8_rows(w2, "gemm_int8 second weight")
+        if w2.q.shape != w.q.shape:
+            raise KernelError("gemm_int8: the two weights of the gated epilogue must agree in shape")
+    bias_code = _vector_code(bias, N, "gemm_int8 bias") if bias is not None else F32
     if epilogue == EPI_ADD and (out is None or out.dtype != torch.float32):
         raise KernelError("gemm_int8: the accumulate epilogue needs an fp32 output to add into")
     if out is not None:
         if out_dtype is not None and out.dtype != out_dtype:
             raise KernelError(f"gemm_int8: output is {out.dtype}, asked for {out_dtype}")
-        _rows2d(out, "gemm_int8 output")
-        if out.shape[0] != M or out.shape[1] != N:
+        _, _, ldo = _own_rows_of(out, "gemm_int8 output")
+        if out.shape != (M, N):
             raise KernelError(f"gemm_int8: output is {tuple(out.shape)}, expected {(M, N)}")
-        _apart(out, "gemm_int8 output")
-    out_code = _code(out.dtype if out is not None else out_dtype or torch.bfloat16)
-    _here(a.q, a.scale, w.q, w.scale, *((w2.q, w2.scale) if w2 is not None else ()), bias, out)
+        out_code = _code(out.dtype)
+    else:
+        out_dtype = out_dtype or torch.bfloat16
+        out_code = _code(out_dtype)
+    _here(a.q, a.scale, w.q, w.scale, bias, out)
+    if gated:
+        _here(w2.q, w2.scale)
     if out is None:
-        out = activation_rows(M, N, out_dtype or torch.bfloat16, a.q.device)
+        out = activation_rows(M, N, out_dtype, a.q.device)
+        ldo = out.stride(0)
     if M == 0 or N == 0:
         return out
-    epilogue = int(epilogue) | (int(gate) << 8)  # the kernels take it apart again and refuse what they do not have
-    head = (_ptr(a.q), _distance(a.q), _ptr(a.scale), _ptr(w.q), _distance(w.q), _ptr(w.scale), _ptr(w2.q) if w2 is not None else None,
-            _distance(w2.q) if w2 is not None else 0, _ptr(w2.scale) if w2 is not None else None, _ptr(bias), bias_code, _ptr(out), out_code,
-            _distance(out), M, N, K, epilogue, float(gate_limit))
-    for kernel, size, parts in _int8_plans(M, N, K, w2 is not None) if K % 16 == 0 else ():
-        sums = torch.empty((parts * M * N * (2 if w2 is not None else 1),), dtype=torch.int32, device=out.device) if parts > 1 else None
-        if _try(kernel, *head, size, parts, _ptr(sums), _stream()):
+    first, second = (w.q.data_ptr(), ldw), (w2.q.data_ptr(), ldw2) if gated else (None, 0)
+    rows = (a.q.data_ptr(), lda)
+    fits = K % 16 == 0 and not (first[0] | ldw) % 16 and (not gated or (ldw2 == ldw and second[0] % 16 == 0))
+    kept = ()  # what is laid out anew, until the launches that read it are made
+    if not fits and -(-K // 16) * 16 <= INT8_MOST_INPUTS and _int8_lay_out_pays(-(-M // 64), N, K, gated):
+        first, *kept = _int8_laid_out(w.q, N, K, ldw)
+        if gated:
+            second, *more = _int8_laid_out(w2.q, N, K, ldw2)
+            kept += more
+        rows, *more = _int8_laid_out(a.q, M, K, lda)
+        kept += more
+        K, fits = first[1], True
+    elif fits and (rows[0] | lda) % 16:
+        rows, *kept = _int8_laid_out(a.q, M, K, lda)
+    # (the kernels take the epilogue and the gate apart again and refuse what they do not have)
+    head = (*rows, a.scale.data_ptr(), *first, w.scale.data_ptr(), *second, w2.scale.data_ptr() if gated else None,
+            bias.data_ptr() if bias is not None else None, bias_code, out.data_ptr(), out_code, ldo, M, N, K, epilogue | gate << 8, gate_limit)
+    for _, kernel, size, parts in _int8_plans(M, N, K, gated) if fits else ():
+        sums = _int8_sums(M, N, gated, parts, out)
+        if _try(kernel, *head, size, parts, None if sums is None else sums.data_ptr(), _stream()):
             return out
     _count("general", "jllm_gemm_int8")
-    _call("jllm_gemm_int8", *head, _stream())
+    _, parts = _int8_general(-(-M // 64), N, K, gated)
+    sums = _int8_sums(M, N, gated, parts, out)
+    _call("jllm_gemm_int8", *head, parts, None if sums is None else sums.data_ptr(), _stream())
     return out
+
+
+def _int8_sums(M: int, N: int, gated: bool, parts: int, out: torch.Tensor) -> Optional[torch.Tensor]:
+    """Where the parts of a cut K leave their sums, of this product alone."""
+    return torch.empty((parts * M * N * (2 if gated else 1),), dtype=torch.int32, device=out.device) if parts > 1 else None
+
+
+def _int8_laid_out(q: torch.Tensor, n: int, width: int, distance: int):
+    """((address, entries between rows), tensor): the rows as the fast kernels take them, with zeros up to a multiple of 16."""
+    padded = -(-width // 16) * 16
+    new = torch.empty((n, padded), dtype=torch.int8, device=q.device)
+    _call("jllm_int8_lay_out", q.data_ptr(), distance, new.data_ptr(), padded, n, width, _stream())
+    return (new.data_ptr(), padded), new
 
 
 INT8_STREAM_MOST_ROWS = 64  # of activations that the weight-streaming kernel takes
@@ -840,8 +885,10 @@ INT8_STREAM_WEIGHTS = (8, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64, 72, 80, 96)  #
 INT8_CUTS = (1, 2, 3, 4, 6, 8)
 INT8_CUT_MIN_K = 512          # of a part
 INT8_CUT_MOST_GROUPS = 640    # workgroups of a cut product: more of them gain nothing
-INT8_STREAM_CUT_US = (1.54, 3.0e-6)  # a cut of K: the second launch, and per sum of a part, of which there are few ...
-INT8_TILE_CUT_US = (2.62, 1.12e-6)   # ... and many
+# A cut of K: the second launch, 1.5 of it for the caller's host, which is what a step of few rows waits for where no graph replays it;
+# and per sum of a part, of which there are few or many
+INT8_STREAM_CUT_US = (3.0, 3.0e-6)
+INT8_TILE_CUT_US = (4.1, 1.12e-6)
 
 
 def _int8_stream_us(M: int, N: int, K: int, weights: int, rows: int, parts: int) -> float:
@@ -906,7 +953,7 @@ def _int8_choices(units: int, N: int, K: int, gated: bool):
     if units <= INT8_STREAM_MOST_ROWS:
         best = min((_int8_stream_us(units, N, K, weights, rows, parts), rows, parts) for rows in INT8_STREAM_WEIGHTS
                    for parts in cuts(-(-N // rows), INT8_CUTS if rows >= 16 else (1,)))
-        return (("jllm_gemm_int8_stream", best[1], best[2]),)
+        return ((best[0], "jllm_gemm_int8_stream", best[1], best[2]),)
     found = []
     for large in (False, True):
         if large and K <= 128:
@@ -915,14 +962,46 @@ def _int8_choices(units: int, N: int, K: int, gated: bool):
                          for parts in cuts(-(-N // (tile % 1000 // weights)) * -(-units // (tile // 1000)), (1,) if gated else INT8_CUTS)))
     found.sort()
     # (the large tiles decline operands of 4 GB: then the others' best)
-    return tuple(("jllm_gemm_int8_large" if tile >= INT8_LARGE_FROM else "jllm_gemm_int8_tiled", tile, parts) for _, tile, parts in found)
+    return tuple((us, "jllm_gemm_int8_large" if tile >= INT8_LARGE_FROM else "jllm_gemm_int8_tiled", tile, parts) for us, tile, parts in found)
 
 
 def _int8_plans(M: int, N: int, K: int, gated: bool):
-    """(entry point, its tile or weight rows, parts of K) of the fast kernels for a product, the cheapest by the estimates first."""
+    """(estimated us, entry point, its tile or weight rows, parts of K) of the fast kernels for a product, the cheapest first."""
     if M <= INT8_STREAM_MOST_ROWS:
         return _int8_choices(8 * next(n for n in INT8_STREAM_LOADS if 8 * n >= M), N, K, gated)
     return _int8_choices(-(-M // 64) * 64, N, K, gated)
+
+
+INT8_GENERAL_CUTS = (1, 2, 3, 4, 6, 8, 12, 16)
+INT8_GENERAL_CUT_US = (3.57, 1.79e-6)
+
+
+@functools.lru_cache(maxsize=8192)
+def _int8_general(tiles64: int, N: int, K: int, gated: bool) -> Tuple[float, int]:
+    """(estimated us, parts of K) of the general kernel for ``tiles64`` times 64 rows: its workgroups of 64 x 64 sums take 0.42 us a stage
+    of 128 for each that a compute unit has. Fitted to 270 times of nine products at 1 to 2,048 rows: 11 % off on average, the cheapest by the
+    estimate 1.2 % behind the best cut on average, 14 % at worst (K whole takes up to three times as long)."""
+    weights = 2 if gated else 1
+    stages, tiles, best = -(-K // 128), -(-N // (64 // weights)) * tiles64, None
+    for parts in INT8_GENERAL_CUTS:
+        if parts > 1 and (K // parts < 256 or tiles * parts > 3000):
+            continue
+        each = -(-stages // parts)
+        us = 3.8 + math.hypot(each * 0.42 * -(-tiles * parts // compute_units()), weights * N * K / 3.96e6)
+        us += INT8_GENERAL_CUT_US[0] + INT8_GENERAL_CUT_US[1] * parts * 64 * tiles64 * N * weights if parts > 1 else 0.0
+        if best is None or us < best[0]:
+            best = (us, parts)
+    return best
+
+
+@functools.lru_cache(maxsize=8192)
+def _int8_lay_out_pays(tiles64: int, N: int, K: int, gated: bool) -> bool:
+    """Whether a product whose weights' rows are no multiples of 16 or begin elsewhere is faster with both operands laid out anew (a
+    launch each: 16.8 MB 7.4 us, 89 MB 29.5, few rows 3.5) than by the general kernel. us, general / so: 512 rows of 4,096 x 12,288 92 / 68, of
+    5,120 x 17,408 167 / 96, 2,048 of them 540 / 190; 256 rows of 4,096 x 12,288 59 / 58; 64 24 / 42."""
+    weights = 2 if gated else 1
+    lay_out = weights * (2.5 + 2.0 * N * K / 6.5e6) + 3.5 + 64 * tiles64 * K / 3.2e6
+    return _int8_plans(64 * tiles64, N, -(-K // 16) * 16, gated)[0][0] + lay_out < _int8_general(tiles64, N, K, gated)[0]
 
 
 MAX_HEAD_DIM = 512     # what the general attention kernel takes (csrc/attention_generic.hip); the fast ones take less

@@ -262,6 +262,36 @@ def test_largest_sums(ops, M, N):
     assert torch.equal(ops.gemm_int8(a_, w_, out_dtype=torch.float32).cpu(), want.expand(M, N))
 
 
+@pytest.mark.parametrize("M,N,K,pad,at,kernel", [
+    (1, 300, 4096, 0, 0, "jllm_gemm_int8_stream"), (64, 300, 4096, 16, 16, "jllm_gemm_int8_stream"), (40, 300, 4096, "a", 3, "jllm_gemm_int8_stream"),
+    (65, 300, 1040, 0, 0, "jllm_gemm_int8_tiled"), (100, 300, 1040, "a", 1, "jllm_gemm_int8_tiled"), (2100, 4096, 2064, 0, 0, "jllm_gemm_int8_large"),
+    (2100, 4096, 2061, 0, 0, "jllm_gemm_int8_large"), (2100, 4096, 2064, 1, 0, "jllm_gemm_int8_large"), (2100, 4096, 2064, 0, 5, "jllm_gemm_int8_large"),
+    (3, 300, 8191, 0, 0, None), (70, 300, 8191, 0, 0, None), (3, 300, 131071, 0, 0, None), (1100, 300, 131071, 0, 0, None), (200, 130, 144, 1, 0, None)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_each_kernel_takes_its_products(ops, M, N, K, pad, at, kernel, gated):
+    """Which kernel a product goes through (None: the general one), with K cut or whole, operands as they lie or laid out anew."""
+    gen = seeded(M + K)
+    a, w, w2 = operands(ops, gen, M, N, K)
+    if pad == "a":  # the activations alone begin anywhere
+        a = ops.Int8Rows(strided(a.q, 0, at)[0], a.scale)
+    elif pad or at:
+        a, w, w2 = (ops.Int8Rows(strided(t.q, pad, at)[0], t.scale) for t in (a, w, w2))
+    ops.reset_stats()
+    if gated:
+        got = ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, out_dtype=torch.float32)
+    else:
+        got = ops.gemm_int8(a, w, out_dtype=torch.float32)
+    ran = ops.stats()
+    assert list(ran["ran"]) == ([kernel] if kernel else []) and list(ran["general"]) == ([] if kernel else ["jllm_gemm_int8"]), ran
+    if gated:
+        z, u = oracle.sums(a, w), oracle.sums(a, w2)
+        y = oracle.gate("silu", z, u)
+        tol = y.abs() * (13 + 6 * z.abs()) * U * 1.01 + 1e-30
+    else:
+        y, tol = oracle.product(a, w)
+    close(got, y, tol)
+
+
 @pytest.mark.parametrize("gate,limit", [("gelu_tanh", 0.0), ("swish_clamped", 1.5)])
 @pytest.mark.parametrize("M,N,K", [(3, 50, 70), (4, 256, 512), (40, 256, 512), (300, 272, 528)])
 def test_gate_functions(ops, gate, limit, M, N, K):
