@@ -678,10 +678,9 @@ class Int8Rows:
         n, width, distance = _int8_rows(self, "rows")
         code = _code(dtype)
         _here(self.q, self.scale)
-        out = activation_rows(n, width, dtype, self.q.device)
+        out = _new_rows(n, width, dtype, self.q)
         if n and width:
-            _call("jllm_dequantize_rows", self.q.data_ptr(), distance, self.scale.data_ptr(), n, width, out.data_ptr(), code, _rows_of(out, "values")[2],
-                  _stream())
+            _call("jllm_dequantize_rows", self.q.data_ptr(), distance, self.scale.data_ptr(), n, width, out.data_ptr(), code, out.stride(0), _stream())
         return out
 
 
@@ -693,6 +692,10 @@ INT8_MOST_INPUTS = 131071  # of a product: 128^2 times as many stay below 2^31, 
 
 def _rows_of(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
     """(rows, width, entries from one row to the next) of a 2-D tensor with contiguous rows; a single row's stride says nothing."""
+    if t.dim() == 2 and t.is_contiguous():
+        n, width = t.shape
+        if n * width < 1 << 31:
+            return n, width, width
     shape, strides = t.shape, t.stride()
     if len(shape) != 2 or strides[1] != 1:
         raise KernelError(f"{what} must be a 2-D tensor with contiguous rows, got shape {tuple(shape)} strides {strides}")
@@ -724,10 +727,10 @@ def _int8_rows(rows: Int8Rows, what: str) -> Tuple[int, int, int]:
     if not isinstance(rows, Int8Rows):
         raise KernelError(f"{what} must be Int8Rows, got {type(rows).__name__}")
     q, scale = rows.q, rows.scale
-    if q.dtype != torch.int8:
+    if q.dtype is not torch.int8:
         raise KernelError(f"{what} must be int8, got {q.dtype}")
     found = _rows_of(q, what)
-    if scale.dtype != torch.float32 or scale.shape != (found[0],) or not scale.is_contiguous():
+    if scale.dtype is not torch.float32 or scale.dim() != 1 or scale.numel() != found[0] or not scale.is_contiguous():
         raise KernelError(f"{what}: the scales must be a contiguous fp32 tensor with one entry per row ({found[0]}), got "
                           f"{scale.dtype} {tuple(scale.shape)}")
     return found
@@ -739,8 +742,13 @@ def _vector_code(t: torch.Tensor, n: int, what: str) -> int:
     return _code(t.dtype)
 
 
-def _new_int8_rows(n: int, width: int, device) -> Int8Rows:
-    return Int8Rows(torch.empty((n, width), dtype=torch.int8, device=device), torch.empty((n,), dtype=torch.float32, device=device))
+def _new_rows(n: int, width: int, dtype: torch.dtype, beside: torch.Tensor) -> torch.Tensor:
+    """``activation_rows`` on the GPU of ``beside``; of few rows in half the time."""
+    return beside.new_empty_strided((n, width), (width, 1), dtype=dtype) if n < PAD_ROWS_FROM else activation_rows(n, width, dtype, beside.device)
+
+
+def _new_int8_rows(n: int, width: int, beside: torch.Tensor) -> Int8Rows:
+    return Int8Rows(beside.new_empty_strided((n, width), (width, 1), dtype=torch.int8), beside.new_empty_strided((n,), (1,), dtype=torch.float32))
 
 
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
@@ -752,7 +760,7 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     if width == 0:
         raise KernelError("quantize_rows: rows without entries have no scale")
     _here(x)
-    out = _new_int8_rows(n, width, x.device)
+    out = _new_int8_rows(n, width, x)
     if n:
         _call("jllm_quantize_rows", x.data_ptr(), code, distance, n, width, out.q.data_ptr(), width, out.scale.data_ptr(), _stream())
     return out
@@ -786,7 +794,7 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
             raise KernelError(f"rmsnorm_int8: the sum goes to an fp32 tensor of x's shape, got {out.dtype} {tuple(out.shape)}")
         joins = (add.data_ptr(), add_code, add_distance, out.data_ptr(), out_distance)
         _here(x, gain, add, out)
-    rows = _new_int8_rows(n, width, x.device)
+    rows = _new_int8_rows(n, width, x)
     if n:
         _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, rows.q.data_ptr(), width,
               rows.scale.data_ptr(), _stream())
@@ -833,7 +841,7 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
     if gated:
         _here(w2.q, w2.scale)
     if out is None:
-        out = activation_rows(M, N, out_dtype, a.q.device)
+        out = _new_rows(M, N, out_dtype, a.q)
         ldo = out.stride(0)
     if M == 0 or N == 0:
         return out
@@ -885,10 +893,9 @@ INT8_STREAM_WEIGHTS = (8, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64, 72, 80, 96)  #
 INT8_CUTS = (1, 2, 3, 4, 6, 8)
 INT8_CUT_MIN_K = 512          # of a part
 INT8_CUT_MOST_GROUPS = 640    # workgroups of a cut product: more of them gain nothing
-# A cut of K: the second launch, 1.5 of it for the caller's host, which is what a step of few rows waits for where no graph replays it;
-# and per sum of a part, of which there are few or many
-INT8_STREAM_CUT_US = (3.0, 3.0e-6)
-INT8_TILE_CUT_US = (4.1, 1.12e-6)
+# A cut of K: the second launch, and per sum of a part, of which there are few or many
+INT8_STREAM_CUT_US = (1.54, 3.0e-6)
+INT8_TILE_CUT_US = (2.62, 1.12e-6)
 
 
 def _int8_stream_us(M: int, N: int, K: int, weights: int, rows: int, parts: int) -> float:
@@ -973,7 +980,7 @@ def _int8_plans(M: int, N: int, K: int, gated: bool):
 
 
 INT8_GENERAL_CUTS = (1, 2, 3, 4, 6, 8, 12, 16)
-INT8_GENERAL_CUT_US = (3.57, 1.79e-6)
+INT8_GENERAL_CUT_US = (3.57, 1.79e-6)  # 1.5 of the launch for the host of a caller without graphs, who waits for it in products as short as these
 
 
 @functools.lru_cache(maxsize=8192)

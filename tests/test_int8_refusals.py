@@ -87,4 +87,4 @@ def test_gemm_int8():
 def test_a_single_row_may_have_any_stride():
     """A row alone has no distance to the next: it is not refused for the stride it happens to have."""
     assert ops._own_rows_of(torch.zeros(8, 1).t(), "row") == (1, 8, 8)
-    refused("2^31", ops._rows_of, torch.zeros(0, dtype=torch.int8).as_strided((2, 0), (1 << 31, 1)), "rows")
+    refused("2^31", ops._rows_of, torch.empty_strided((2, 1), (1 << 31, 1), dtype=torch.int8, device="meta"), "rows")
