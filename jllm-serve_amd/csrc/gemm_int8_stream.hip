@@ -53,6 +53,9 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
   const int n0 = blockIdx.x * p.rows;
   const int first = blockIdx.y * p.blocks, nblk = min((p.K + 127) / 128 - first, p.blocks);
   const int tail = p.K & 127;  // bytes of the last block of K, where it is not whole
+  // workgroups walk K from different blocks, so that they do not all ask the same memory channels at once (rows often lie a multiple of
+  // 4 KB apart; us, from the first block / so: 1 x 4,096 x 4,096 6.1 / 5.4, 8 x 12,288 x 4,096 gated 21.3 / 20.4, 8 x 4,096 x 12,288 12.2 / 11.1)
+  const int turn = (int)((blockIdx.x * 3u) % (unsigned)nblk);
   // ---- the loads of a block: a scalar base that advances with the block and a byte offset per lane that never changes
   uint32_t goff[NI];
   const int lrow = lane >> 3, lslot = lane & 7;
@@ -69,7 +72,8 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)ring;
   const int total = wave < nblk ? (nblk - wave + WAVES - 1) / WAVES : 0;
   auto issue = [&](int i, int slot) {
-    const int b = first + wave + i * WAVES;
+    int b = wave + i * WAVES + turn;
+    b = first + (b >= nblk ? b - nblk : b);
     const size_t kbytes = (size_t)b * 128;
     const bool cut = tail != 0 && (b + 1) * 128 > p.K;
 #pragma unroll
@@ -160,8 +164,8 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (c >= there) continue;
-        const float z = ((float)sum[0][c] * sa) * p.end.scales.w[n + c] + int8_bias(p.end, n + c);
-        y[c] = GATED ? gated<true>(z, ((float)sum[MATS - 1][c] * sa) * p.end.scales.w2[n + c], p.end.gate) : z;
+        const float z = int8_output(sum[0][c], sa, p.end.scales.w[n + c], int8_bias(p.end, n + c));
+        y[c] = GATED ? gated<true>(z, int8_output(sum[MATS - 1][c], sa, p.end.scales.w2[n + c], 0.f), p.end.gate) : z;
       }
       int8_store4(p.end, m, n, there, vec, y);
     }

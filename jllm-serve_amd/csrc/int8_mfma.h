@@ -40,6 +40,14 @@ __device__ __forceinline__ float int8_bias(const Int8Epilogue& p, int n) {
   return !p.bias ? 0.f : p.bias_dtype == JLLM_BF16 ? ldf((const bf16_t*)p.bias, n) : ldf((const float*)p.bias, n);
 }
 
+// A sum with its scales and bias. Every kernel rounds here alike (no product joined with an addition), so that a row's outputs have the same
+// bits from all of them.
+__device__ __forceinline__ float int8_output(int sum, float sa, float sw, float b) {
+#pragma clang fp contract(off)
+  const float y = ((float)sum * sa) * sw;
+  return y + b;
+}
+
 // Four neighbouring outputs of row m from column n on, of which `there` exist; `vec`: the row's places from n on are 16-byte aligned (8 in bf16)
 __device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n, int there, bool vec, floatx4 v) {
   const size_t o = (size_t)m * p.ldo + n;
@@ -94,8 +102,8 @@ __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int la
       floatx4 v;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float z = ((float)acc[i][j][c] * sa) * sw[j][c] + bv[j][c];
-        v[c] = GATED ? gated<true>(z, ((float)acc[i][GATED ? NI + j : 0][c] * sa) * su[j][c], p.gate) : z;
+        const float z = int8_output(acc[i][j][c], sa, sw[j][c], bv[j][c]);
+        v[c] = GATED ? gated<true>(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa, su[j][c], 0.f), p.gate) : z;
       }
       return v;
     };

@@ -213,7 +213,7 @@ int launch_rows(const RowsArgs& a, int rows, hipStream_t stream) {
 
 extern "C" int jllm_quantize_rows(const void* x, int dtype, int ldx, int rows, int width, void* q, int ldq, float* scale, hipStream_t stream) {
   if (rows <= 0) return 0;
-  if (width <= 0 || ldx < 0 || ldq < width) JLLM_FAIL("quantize_rows: rows of %d, %d and %d apart", width, ldx, ldq);
+  if (width <= 0 || width > (1 << 30) || ldx < 0 || ldq < width) JLLM_FAIL("quantize_rows: rows of %d, %d and %d apart", width, ldx, ldq);
   RowsArgs a{x, nullptr, nullptr, nullptr, (signed char*)q, scale, ldx, 0, 0, ldq, width, 0.f};
   JLLM_DISPATCH_1(dtype, T, { return (launch_rows<false, false, T, float, float>(a, rows, stream)); })
 }
@@ -221,7 +221,7 @@ extern "C" int jllm_quantize_rows(const void* x, int dtype, int ldx, int rows, i
 extern "C" int jllm_rmsnorm_int8(const float* x, int ldx, const void* add, int add_dtype, int ld_add, float* sum, int ld_sum, int rows, int width,
                                  const void* gain, int gain_dtype, float eps, void* q, int ldq, float* scale, hipStream_t stream) {
   if (rows <= 0) return 0;
-  if (width <= 0 || ldx < 0 || ldq < width) JLLM_FAIL("rmsnorm_int8: rows of %d, %d and %d apart", width, ldx, ldq);
+  if (width <= 0 || width > (1 << 30) || ldx < 0 || ldq < width) JLLM_FAIL("rmsnorm_int8: rows of %d, %d and %d apart", width, ldx, ldq);
   if ((add != nullptr) != (sum != nullptr)) JLLM_FAIL("rmsnorm_int8: rows to add and a place for the sum come together");
   if (add && (ld_add < 0 || ld_sum < width)) JLLM_FAIL("rmsnorm_int8: sums %d apart for rows of %d", ld_sum, width);
   RowsArgs a{x, add, gain, sum, (signed char*)q, scale, ldx, ld_add, ld_sum, ldq, width, eps};
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const signed char*
 
 extern "C" int jllm_dequantize_rows(const void* q, int ldq, const float* scale, int rows, int width, void* out, int out_dtype, int ldo, hipStream_t stream) {
   if (rows <= 0) return 0;
-  if (width <= 0 || ldq < 0 || ldo < width) JLLM_FAIL("dequantize_rows: rows of %d, %d and %d apart", width, ldq, ldo);
+  if (width <= 0 || width > (1 << 30) || ldq < 0 || ldo < width) JLLM_FAIL("dequantize_rows: rows of %d, %d and %d apart", width, ldq, ldo);
   const int v = width < 8 ? 1 : 8, pieces = (width + v - 1) / v;
   const size_t groups = ((size_t)rows * pieces + 255) / 256;
   if (groups > 0x7fffffffull) JLLM_FAIL("dequantize_rows: %d rows of %d are more than a grid takes", rows, width);

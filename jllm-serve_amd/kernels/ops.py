@@ -701,17 +701,17 @@ def _rows_of(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
         raise KernelError(f"{what} must be a 2-D tensor with contiguous rows, got shape {tuple(shape)} strides {strides}")
     n, width = shape
     distance = strides[0] if n > 1 else width
-    if distance >= 1 << 31 or n >= 1 << 31:
+    if distance >= 1 << 31 or n >= 1 << 31:  # (and so may be the width of a single row)
         raise KernelError(f"{what}: the kernels take fewer than 2^31 rows, less than 2^31 entries apart; got {tuple(shape)}, strides {strides}")
     return n, width, distance
 
 
 def _own_rows_of(t: torch.Tensor, what: str) -> Tuple[int, int, int]:
     """The same of rows that are written: none over another."""
-    found = _rows_of(t, what)
-    if found[2] < found[1]:
+    n, width, distance = _rows_of(t, what)
+    if distance < width:
         raise KernelError(f"{what} must have rows of their own, got shape {tuple(t.shape)} strides {t.stride()}")
-    return found
+    return n, width, distance
 
 
 def _here(*tensors) -> None:
@@ -770,7 +770,8 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
                  out: Optional[torch.Tensor] = None) -> Int8Rows:
     """RMSNorm of fp32 rows of ``x`` with ``gain`` as 8-bit rows for ``gemm_int8`` (scales and rounding as ``quantize_rows``; the norm
     itself is not rounded in between). With ``add`` (fp32 or bf16, of x's shape), what a sublayer leaves, the norm is that of
-    ``x + add``, and the sum goes to ``out`` (fp32; not given: into ``x``, the residual stream)."""
+    ``x + add``, and the sum goes to ``out`` (fp32; not given: into ``x``, the residual stream): x or add itself, or rows that share no
+    memory with them."""
     if x.dtype != torch.float32:
         raise KernelError("rmsnorm_int8 takes fp32 rows")
     n, width, distance = _rows_of(x, "rmsnorm_int8 input")
@@ -783,14 +784,14 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
         joins = (None, F32, 0, None, 0)
         _here(x, gain)
     else:
-        _, _, add_distance = _rows_of(add, "rmsnorm_int8 rows to add")
-        if add.shape != x.shape:
+        add_n, add_width, add_distance = _rows_of(add, "rmsnorm_int8 rows to add")
+        if add_n != n or add_width != width:
             raise KernelError(f"rmsnorm_int8: rows to add {tuple(add.shape)} for {tuple(x.shape)}")
         add_code = _code(add.dtype)
         if out is None:
             out = x
-        _, _, out_distance = _own_rows_of(out, "rmsnorm_int8 sum")
-        if out.dtype != torch.float32 or out.shape != x.shape:
+        out_n, out_width, out_distance = _own_rows_of(out, "rmsnorm_int8 sum")
+        if out.dtype != torch.float32 or out_n != n or out_width != width:
             raise KernelError(f"rmsnorm_int8: the sum goes to an fp32 tensor of x's shape, got {out.dtype} {tuple(out.shape)}")
         joins = (add.data_ptr(), add_code, add_distance, out.data_ptr(), out_distance)
         _here(x, gain, add, out)
@@ -830,8 +831,8 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
     if out is not None:
         if out_dtype is not None and out.dtype != out_dtype:
             raise KernelError(f"gemm_int8: output is {out.dtype}, asked for {out_dtype}")
-        _, _, ldo = _own_rows_of(out, "gemm_int8 output")
-        if out.shape != (M, N):
+        rows, columns, ldo = _own_rows_of(out, "gemm_int8 output")
+        if rows != M or columns != N:
             raise KernelError(f"gemm_int8: output is {tuple(out.shape)}, expected {(M, N)}")
         out_code = _code(out.dtype)
     else:

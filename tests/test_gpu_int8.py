@@ -162,6 +162,21 @@ def test_rmsnorm_int8(ops, width, adt, gdt):
         assert torch.equal(xbig, kept)  # nothing between the rows or behind them was written
 
 
+@pytest.mark.parametrize("width", [5, 40, 100, 1031, 5120, 20000, 33000])
+def test_norm_of_a_sum_of_shared_rows(ops, width):
+    """The rows to add may be x itself, and the sum may go into them."""
+    gen = seeded(width)
+    x, add, g = normal(gen, 6, width), normal(gen, 6, width), normal(gen, width)
+    want, place = ops.rmsnorm_int8(x, g, 1e-6, add=add, out=torch.empty_like(x)), x + add
+    into = add.clone()
+    got = ops.rmsnorm_int8(x, g, 1e-6, add=into, out=into)
+    assert torch.equal(got.q, want.q) and torch.equal(got.scale, want.scale) and torch.equal(into, place)
+    twice = x.clone()
+    got = ops.rmsnorm_int8(twice, g, 1e-6, add=twice)
+    want = ops.rmsnorm_int8(2 * x, g, 1e-6)
+    assert torch.equal(got.q, want.q) and torch.equal(got.scale, want.scale) and torch.equal(twice, 2 * x)
+
+
 def test_norm_of_rows_beside_others(ops):
     """A row's bits do not depend on the rows beside it."""
     gen = seeded(2)
@@ -292,6 +307,59 @@ def test_each_kernel_takes_its_products(ops, M, N, K, pad, at, kernel, gated):
     close(got, y, tol)
 
 
+TILES = [("jllm_gemm_int8_tiled", t) for t in (64064, 64128, 128128)] + [("jllm_gemm_int8_large", t) for t in (128256, 256128, 192256, 256256)]
+
+
+@pytest.mark.parametrize("kernel,tile", TILES)
+@pytest.mark.parametrize("K", [144, 256, 400, 640, 656, 1040, 2176, 2192])
+def test_every_tile(ops, monkeypatch, kernel, tile, K):
+    """Each tile by name, at numbers of whole and cut stages around its ring's depth, K whole and in parts, with rows and columns that end inside a
+    tile: the bits of the general kernel."""
+    gen = seeded(tile + K)
+    for M, N in ((1, 5), (70, 300), (300, 130), (513, 520)):
+        a, w, w2 = operands(ops, gen, M, N, K)
+        bias, base = normal(gen, N), normal(gen, M, N)
+        monkeypatch.setattr(ops, "_int8_plans", lambda *args: ())
+        want = ops.gemm_int8(a, w, bias=bias, out_dtype=torch.float32)
+        narrow = ops.gemm_int8(a, w)
+        gated = ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, out_dtype=torch.float32)
+        added = ops.gemm_int8(a, w, out=base.clone(), epilogue=ops.EPI_ADD)
+        for parts in (1, 2, 3, 5):
+            stages = -(-K // 128)
+            if parts > 1 and stages <= -(-stages // parts) * (parts - 1):
+                continue  # a part without any
+            monkeypatch.setattr(ops, "_int8_plans", lambda *args: ((0.0, kernel, tile, parts),))
+            ops.reset_stats()
+            assert torch.equal(ops.gemm_int8(a, w, bias=bias, out_dtype=torch.float32), want)
+            assert torch.equal(ops.gemm_int8(a, w), narrow)
+            assert torch.equal(ops.gemm_int8(a, w, out=base.clone(), epilogue=ops.EPI_ADD), added)
+            assert ops.stats()["ran"] == {kernel: 3}
+            if parts == 1:
+                assert torch.equal(ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, out_dtype=torch.float32), gated)
+
+
+@pytest.mark.parametrize("M", [1, 8, 9, 30, 48, 64])
+@pytest.mark.parametrize("K", [16, 128, 144, 1040, 2176, 8208])
+def test_every_number_of_weight_rows(ops, monkeypatch, M, K):
+    """The weight-streaming kernel at every number of weight rows per workgroup, K whole and in parts: the bits of the general kernel."""
+    gen = seeded(M + K)
+    N = 203
+    a, w, w2 = operands(ops, gen, M, N, K)
+    base = normal(gen, M, N)
+    monkeypatch.setattr(ops, "_int8_plans", lambda *args: ())
+    want = ops.gemm_int8(a, w)
+    gated = ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED)
+    added = ops.gemm_int8(a, w, out=base.clone(), epilogue=ops.EPI_ADD)
+    for rows in (1, 3, 8, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64, 72, 80, 96):
+        for parts in (1, 2, 4, 7):
+            monkeypatch.setattr(ops, "_int8_plans", lambda *args: ((0.0, "jllm_gemm_int8_stream", rows, parts),))
+            ops.reset_stats()
+            assert torch.equal(ops.gemm_int8(a, w), want)
+            assert torch.equal(ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED), gated)
+            assert torch.equal(ops.gemm_int8(a, w, out=base.clone(), epilogue=ops.EPI_ADD), added)
+            assert ops.stats()["ran"] == {"jllm_gemm_int8_stream": 3}
+
+
 @pytest.mark.parametrize("gate,limit", [("gelu_tanh", 0.0), ("swish_clamped", 1.5)])
 @pytest.mark.parametrize("M,N,K", [(3, 50, 70), (4, 256, 512), (40, 256, 512), (300, 272, 528)])
 def test_gate_functions(ops, gate, limit, M, N, K):
@@ -311,17 +379,18 @@ def test_gate_functions(ops, gate, limit, M, N, K):
 
 
 def test_a_row_has_the_same_bits_in_any_batch(ops):
+    """Whatever kernel, tile and cut the number of rows leads to, with every epilogue."""
     gen = seeded(11)
-    a, w, w2 = operands(ops, gen, 700, 640, 1152)
-    whole, gated = ops.gemm_int8(a, w, out_dtype=torch.float32), ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, out_dtype=torch.float32)
-    for n in (1, 5, 16, 17, 33, 64, 65, 128, 200, 257, 513):
-        part = ops.Int8Rows(a.q[3:3 + n], a.scale[3:3 + n])
-        assert torch.equal(ops.gemm_int8(part, w, out_dtype=torch.float32), whole[3:3 + n])
-        got = ops.gemm_int8(part, w, w2=w2, epilogue=ops.EPI_GATED, out_dtype=torch.float32)
-        y = oracle.gate("silu", oracle.sums(part, w), oracle.sums(part, w2))
-        z = oracle.sums(part, w)
-        tol = y.abs() * (13 + 6 * z.abs()) * U * 1.01 + 1e-30
-        close(got, y, tol)
+    a, w, w2 = operands(ops, gen, 1200, 640, 1152)
+    bias, base = normal(gen, 640), normal(gen, 1200, 640)
+    calls = [lambda part, rows: ops.gemm_int8(part, w, bias=bias, out_dtype=torch.float32), lambda part, rows: ops.gemm_int8(part, w),
+             lambda part, rows: ops.gemm_int8(part, w, w2=w2, epilogue=ops.EPI_GATED, out_dtype=torch.float32),
+             lambda part, rows: ops.gemm_int8(part, w, bias=bias, out=base[rows].clone(), epilogue=ops.EPI_ADD)]
+    whole = [call(a, slice(0, 1200)) for call in calls]
+    for n in (1, 5, 16, 17, 33, 64, 65, 128, 200, 257, 513, 1100):
+        rows = slice(3, 3 + n)
+        for call, want in zip(calls, whole):
+            assert torch.equal(call(ops.Int8Rows(a.q[rows], a.scale[rows]), rows), want[rows]), n
 
 
 def test_no_rows_and_no_outputs(ops):
