@@ -11,7 +11,7 @@
 #include <type_traits>
 #include "int8_mfma.h"
 #include "int8_parts.h"
-#include "pingpong_tile.h"
+#include "lds_ring.h"
 
 #define T8_ROW_BYTES 128
 #define T8_FENCE() __builtin_amdgcn_sched_barrier(0)
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(WGM* WGN * 64) void gemm_int8_tiled_kernel(Int8Args
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int wm = wave / WGN, wn = wave % WGN;
   int row, col;
-  die_tile(blockIdx.x + blockIdx.y * gridDim.x, gridDim.y, gridDim.x, row, col);
+  int8_die_tile(blockIdx.x + blockIdx.y * gridDim.x, gridDim.y, gridDim.x, row, col);
   const int m0 = row * TBM, n0 = col * (GATED ? TBN / 2 : TBN);
   const int nk_all = (p.K + 127) / 128, nk_per = (nk_all + gridDim.z - 1) / gridDim.z, kt0 = blockIdx.z * nk_per;
   const int nk = max(0, min(nk_all, kt0 + nk_per) - kt0);

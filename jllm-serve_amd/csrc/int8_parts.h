@@ -10,6 +10,16 @@ struct Int8Args {
   Int8Epilogue end;
 };
 
+// Which tile workgroup b of rows x cols takes: workgroups b, b + 8, b + 16 .. share a die, which gets a run of neighbouring tiles, in
+// bands of four columns, row by row inside a band, so that its L2 passes on fewer operands
+__device__ __forceinline__ void int8_die_tile(int b, int rows, int cols, int& row, int& col) {
+  const int tiles = rows * cols, each = tiles >> 3, more = tiles & 7, die = b & 7;
+  const int i = die * each + min(die, more) + (b >> 3);
+  const int band = i / (4 * rows), r = i - band * 4 * rows, width = min(4, cols - band * 4);
+  row = r / width;
+  col = band * 4 + r - row * width;
+}
+
 // four neighbouring sums of row m from column n on, of which `there` exist
 __device__ __forceinline__ void int8_part_store(int* __restrict__ part, int m, int n, int there, int N, intx4 v) {
   int* to = part + (size_t)m * N + n;
