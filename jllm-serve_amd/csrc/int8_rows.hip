@@ -2,7 +2,7 @@
 // between two sublayers, and read back.
 //
 //   most = max_i |y[i]|,  scale = most / 127,  q[i] = round(y[i] * (127 / most)), halves to even, -127 .. 127
-//   norm: h = x + add (fp32, written), y = (h * r) * gain, r = 1 / sqrt(mean(h^2) + eps) (norm_scale of common.h)
+//   norm: h = x + add (fp32, written), y = (h * r) * gain, r = 1 / sqrt(mean(h^2) + eps)
 //
 // A row of zeros has scale 0 and zeros. A row with a NaN or an infinity has scale NaN and zeros, so that everything computed
 // from it is NaN. Rows whose largest value lies below 2^-100 are multiplied by 2^100 first (exact), where 127 / most
@@ -47,12 +47,13 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 }
 
 template <int NW>
-__device__ __forceinline__ float row_sum(float v, float* red) {  // in a fixed order; `red` is this reduction's alone
-  v = wave_sum(v);
+__device__ __forceinline__ double row_sum(double v, double* red) {  // in a fixed order; `red` is this reduction's alone
+#pragma unroll
+  for (int o = JLLM_WAVE / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, JLLM_WAVE);
   if (NW == 1) return v;
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  float s = 0.f;
+  double s = 0.0;
 #pragma unroll
   for (int i = 0; i < NW; ++i) s += red[i];
   return s;
@@ -89,13 +90,17 @@ __device__ __forceinline__ uint32_t rounded(float y, const Rounding& r) {
   return r.inv == 0.f ? 0u : __float_as_uint(t + 12582912.0f) & 0xffu;
 }
 
+// The norm's scale. Squares and their sum are in 64 bits, where the squares are exact and none overflows: the kernel waits for memory
+// meanwhile, and a scale that is off by one unit turns whole numbers that lie near a half.
+__device__ __forceinline__ float rms_scale(double squares, int n, float eps) { return (float)(1.0 / sqrt(squares / n + (double)eps)); }
+
 // Every entry of a norm is (h * r) * gain, two roundings
 __device__ __forceinline__ float normed(float h, float r, float g) { return (h * r) * g; }
 
 template <bool NORM, bool ADD, typename TX, typename TA, typename TG, int J, int THREADS>
 __global__ __launch_bounds__(THREADS) void int8_rows_kernel(RowsArgs p) {
   constexpr int NW = THREADS / 64;
-  __shared__ float red_sum[NW];
+  __shared__ double red_sum[NW];
   __shared__ uint32_t red_max[NW];
   const size_t row = blockIdx.x;
   const TX* x = (const TX*)p.x + row * p.ldx;
@@ -126,17 +131,18 @@ __global__ __launch_bounds__(THREADS) void int8_rows_kernel(RowsArgs p) {
     if (NORM) {
 #pragma unroll
       for (int j = 0; j < J; ++j) load8(gain + at[j], g[j]);
-      float ss = 0.f;
+      double ss = 0.0;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int first = (tid + THREADS * j) * 8;  // what lies below it in the piece belongs to the one before
-        float s = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += at[j] + e >= first ? v[j][e] * v[j][e] : 0.f;
-        ss += s;
+        for (int e = 0; e < 8; ++e) {
+          const double h = at[j] + e >= first ? v[j][e] : 0.f;
+          ss += h * h;
+        }
       }
       ss = row_sum<NW>(ss, red_sum);
-      const float r = norm_scale(ss, d, p.eps);
+      const float r = rms_scale(ss, d, p.eps);
       if (ADD) {  // behind the barrier: every thread has its overlapping entries of the old row
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -169,16 +175,16 @@ __global__ __launch_bounds__(THREADS) void int8_rows_kernel(RowsArgs p) {
     // A row of any width, entry by entry; a thread reads again what it alone wrote
     float r = 0.f;
     if (NORM) {
-      float ss = 0.f;
+      double ss = 0.0;
       for (int i = tid; i < d; i += THREADS) {
         float h = ldf(x, i);
         if (ADD) {
           h += ldf(add, i);
           sum[i] = h;
         }
-        ss += h * h;
+        ss += (double)h * h;
       }
-      r = norm_scale(row_sum<NW>(ss, red_sum), d, p.eps);
+      r = rms_scale(row_sum<NW>(ss, red_sum), d, p.eps);
     }
     auto entry = [&](int i) { return NORM ? normed(ADD ? sum[i] : ldf(x, i), r, ldf(gain, i)) : ldf(x, i); };
     uint32_t most = 0;

@@ -40,9 +40,9 @@ def strided(x, pad, at=0):
 WIDTHS = [1, 3, 7, 8, 9, 15, 16, 64, 100, 505, 512, 520, 1000, 1024, 1031, 2048, 2055, 4096, 5120, 5123, 6151, 8192, 8200, 12288, 17408, 25600, 32768, 32771, 40000]
 
 
-def terms(width):
-    """Most additions that a norm's sum of squares goes through, for the tolerance of its scale: a thread's own, the wave's six, the waves'."""
-    return width / 256 + 8 + 6 + 16 if width > 32768 or width < 8 else 32 + 6 + 16
+# fp32 roundings of a norm's scale: the inverse root (its sum is in 64 bits), two products, the quotient; and of an entry against the row's
+# largest, where the inverse root cancels: two products each, the quotient 127 / largest, the last product
+NORM_SCALE, NORM_ENTRY = 5, 6
 
 
 # ------------------------------------------------------------------------------------------------ rows made 8-bit
@@ -120,7 +120,7 @@ def test_numbers_of_rows(ops, rows):
     assert normed.tensor(torch.bfloat16).shape == (rows, 264)
     if rows:
         oracle.check_rows(got.q, got.scale, x, 2, 1)
-        oracle.check_rows(normed.q, normed.scale, oracle.norm(x, torch.ones(264), 1e-6)[1], 8, terms(264) / 2 + 6)
+        oracle.check_rows(normed.q, normed.scale, oracle.norm(x, torch.ones(264), 1e-6)[1], NORM_ENTRY, NORM_SCALE)
 
 
 # ------------------------------------------------------------------------------------------------ the norm
@@ -138,13 +138,11 @@ def test_rmsnorm_int8(ops, width, adt, gdt):
         add = normal(gen, 5, width).to(adt)
         add[2] = 0
     h, y = oracle.norm(x, gain, 1e-5, add)
-    # roundings that do not cancel between an entry and the row's largest: two products each, the largest's quotient, the last product
-    t_roundings, scale_roundings = 6, terms(width) / 2 + 6
     before = x.clone()
     place = torch.empty_like(x) if add is not None else None
     got = ops.rmsnorm_int8(x, gain, 1e-5, add=add, out=place)
     assert torch.equal(x, before)
-    oracle.check_rows(got.q, got.scale, y, t_roundings, scale_roundings)
+    oracle.check_rows(got.q, got.scale, y, NORM_ENTRY, NORM_SCALE)
     assert float(got.scale[2]) == 0 and not got.q[2].any()
     if add is not None:
         assert torch.equal(place.cpu(), h)
@@ -175,6 +173,16 @@ def test_norm_of_a_sum_of_shared_rows(ops, width):
     got = ops.rmsnorm_int8(twice, g, 1e-6, add=twice)
     want = ops.rmsnorm_int8(2 * x, g, 1e-6)
     assert torch.equal(got.q, want.q) and torch.equal(got.scale, want.scale) and torch.equal(twice, 2 * x)
+
+
+@pytest.mark.parametrize("width", [40, 5120, 33000])
+def test_norm_of_large_and_small_rows(ops, width):
+    """Rows whose squares fp32 does not hold: beyond 1e38, and below 1e-45 with an eps as small."""
+    gen = seeded(width)
+    x = normal(gen, 4, width).clamp(-4, 4) * torch.tensor([1e30, 1e-30, 3e37, 1.0], device=DEV)[:, None]
+    g = 1 + 0.1 * normal(gen, width)
+    got = ops.rmsnorm_int8(x, g, 1e-38)
+    oracle.check_rows(got.q, got.scale, oracle.norm(x, g, float(torch.tensor(1e-38)))[1], NORM_ENTRY, NORM_SCALE)
 
 
 def test_norm_of_rows_beside_others(ops):
@@ -422,7 +430,7 @@ def test_a_feed_forward_of_8_bit_rows(ops, rows, width, inner):
     n, hidden, out = feed_forward(ops, x, attended, gain, gate, up, down)
     # every step against the formula on the step's own inputs
     h, y = oracle.norm(x0, gain, 1e-6, attended)
-    oracle.check_rows(n.q, n.scale, y, 6, terms(width) / 2 + 6)
+    oracle.check_rows(n.q, n.scale, y, NORM_ENTRY, NORM_SCALE)
     z, u = oracle.sums(n, gate), oracle.sums(n, up)
     want = oracle.gate("silu", z, u)
     close(hidden, want, oracle.stored(want.abs() * (13 + 6 * z.abs()) * U * 1.01 + 1e-30, want, torch.bfloat16))
