@@ -662,25 +662,47 @@ def gemm(a: torch.Tensor, w: torch.Tensor, *, w2: Optional[torch.Tensor] = None,
 class Int8Rows:
     """Rows of 8-bit integers: ``q`` (int8 [n, width], rows contiguous, any distance apart) and one fp32 ``scale`` per row [n]; row r
     stands for ``q[r] * scale[r]``. Activations are such rows by token, a weight [N, K] by output channel. Made by
-    ``quantize_rows`` and ``rmsnorm_int8``, or from tensors at hand."""
+    ``quantize_rows`` and ``rmsnorm_int8``, or from tensors at hand, which are looked over here, once, and keep their sizes from then on."""
 
-    __slots__ = ("q", "scale")
+    __slots__ = ("_q", "_scale", "_sizes")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
-        self.q, self.scale = q, scale
+        if q.dtype is not torch.int8:
+            raise KernelError(f"8-bit rows must be int8, got {q.dtype}")
+        self._q, self._scale, self._sizes = q, scale, _rows_of(q, "8-bit rows")
+        n = self._sizes[0]
+        if scale.dtype is not torch.float32 or scale.dim() != 1 or scale.numel() != n or not scale.is_contiguous():
+            raise KernelError(f"8-bit rows: the scales must be a contiguous fp32 tensor with one entry per row ({n}), got "
+                              f"{scale.dtype} {tuple(scale.shape)}")
+
+    @classmethod
+    def _new(cls, n: int, width: int, beside: torch.Tensor) -> "Int8Rows":
+        rows = cls.__new__(cls)
+        rows._q = beside.new_empty_strided((n, width), (width, 1), dtype=torch.int8)
+        rows._scale = beside.new_empty_strided((n,), (1,), dtype=torch.float32)
+        rows._sizes = (n, width, width)
+        return rows
+
+    @property
+    def q(self) -> torch.Tensor:
+        return self._q
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._scale
 
     @property
     def shape(self):
-        return self.q.shape
+        return self._q.shape
 
     def tensor(self, dtype: torch.dtype) -> torch.Tensor:
         """The values that the rows stand for, rounded once to ``dtype``."""
-        n, width, distance = _int8_rows(self, "rows")
         code = _code(dtype)
-        _here(self.q, self.scale)
-        out = _new_rows(n, width, dtype, self.q)
+        q, scale, (n, width, distance) = self._q, self._scale, self._sizes
+        _here(q, scale)
+        out = _new_rows(n, width, dtype, q)
         if n and width:
-            _call("jllm_dequantize_rows", self.q.data_ptr(), distance, self.scale.data_ptr(), n, width, out.data_ptr(), code, out.stride(0), _stream())
+            _call("jllm_dequantize_rows", q.data_ptr(), distance, scale.data_ptr(), n, width, out.data_ptr(), code, out.stride(0), _stream())
         return out
 
 
@@ -724,16 +746,9 @@ def _here(*tensors) -> None:
 
 
 def _int8_rows(rows: Int8Rows, what: str) -> Tuple[int, int, int]:
-    if not isinstance(rows, Int8Rows):
+    if type(rows) is not Int8Rows:
         raise KernelError(f"{what} must be Int8Rows, got {type(rows).__name__}")
-    q, scale = rows.q, rows.scale
-    if q.dtype is not torch.int8:
-        raise KernelError(f"{what} must be int8, got {q.dtype}")
-    found = _rows_of(q, what)
-    if scale.dtype is not torch.float32 or scale.dim() != 1 or scale.numel() != found[0] or not scale.is_contiguous():
-        raise KernelError(f"{what}: the scales must be a contiguous fp32 tensor with one entry per row ({found[0]}), got "
-                          f"{scale.dtype} {tuple(scale.shape)}")
-    return found
+    return rows._sizes
 
 
 def _vector_code(t: torch.Tensor, n: int, what: str) -> int:
@@ -747,10 +762,6 @@ def _new_rows(n: int, width: int, dtype: torch.dtype, beside: torch.Tensor) -> t
     return beside.new_empty_strided((n, width), (width, 1), dtype=dtype) if n < PAD_ROWS_FROM else activation_rows(n, width, dtype, beside.device)
 
 
-def _new_int8_rows(n: int, width: int, beside: torch.Tensor) -> Int8Rows:
-    return Int8Rows(beside.new_empty_strided((n, width), (width, 1), dtype=torch.int8), beside.new_empty_strided((n,), (1,), dtype=torch.float32))
-
-
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """Rows of ``x`` (fp32 or bf16 [n, width], any distance apart) as 8-bit integers: scale = max |x| / 127, q = x * (127 / max |x|)
     rounded to the nearest whole number, halves to even. A row of zeros has scale 0; one with a NaN or an infinity has scale NaN
@@ -760,10 +771,10 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     if width == 0:
         raise KernelError("quantize_rows: rows without entries have no scale")
     _here(x)
-    out = _new_int8_rows(n, width, x)
+    rows = Int8Rows._new(n, width, x)
     if n:
-        _call("jllm_quantize_rows", x.data_ptr(), code, distance, n, width, out.q.data_ptr(), width, out.scale.data_ptr(), _stream())
-    return out
+        _call("jllm_quantize_rows", x.data_ptr(), code, distance, n, width, rows._q.data_ptr(), width, rows._scale.data_ptr(), _stream())
+    return rows
 
 
 def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Optional[torch.Tensor] = None,
@@ -795,10 +806,10 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
             raise KernelError(f"rmsnorm_int8: the sum goes to an fp32 tensor of x's shape, got {out.dtype} {tuple(out.shape)}")
         joins = (add.data_ptr(), add_code, add_distance, out.data_ptr(), out_distance)
         _here(x, gain, add, out)
-    rows = _new_int8_rows(n, width, x)
+    rows = Int8Rows._new(n, width, x)
     if n:
-        _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, rows.q.data_ptr(), width,
-              rows.scale.data_ptr(), _stream())
+        _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, rows._q.data_ptr(), width,
+              rows._scale.data_ptr(), _stream())
     return rows
 
 
@@ -816,75 +827,79 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
         raise KernelError(f"gemm_int8: input rows have {K} entries, weight rows {inputs}")
     if not 0 < K <= INT8_MOST_INPUTS:
         raise KernelError(f"gemm_int8: rows of {K} entries (1 to {INT8_MOST_INPUTS}: beyond, the sums could leave 32 bits)")
-    if epilogue not in (EPI_STORE, EPI_ADD, EPI_GATED) or (epilogue == EPI_GATED) != (w2 is not None):
-        raise KernelError("gemm_int8: the gated epilogue takes exactly two weights")
-    if gate and (epilogue != EPI_GATED or not 0 < gate < (1 << 20)):
-        raise KernelError(f"gemm_int8: gate function {gate} without the gated epilogue")
     gated = w2 is not None
+    if gated != (epilogue == EPI_GATED) or epilogue not in (EPI_STORE, EPI_ADD, EPI_GATED):
+        raise KernelError("gemm_int8: the gated epilogue takes exactly two weights")
+    aq, a_scale, wq, w_scale, uq, u_scale, ldu = a._q, a._scale, w._q, w._scale, None, None, 0
     if gated:
-        _, _, ldw2 = _int8_rows(w2, "gemm_int8 second weight")
-        if w2.q.shape != w.q.shape:
+        outputs, inputs, ldu = _int8_rows(w2, "gemm_int8 second weight")
+        if outputs != N or inputs != K:
             raise KernelError("gemm_int8: the two weights of the gated epilogue must agree in shape")
+        uq, u_scale = w2._q, w2._scale
+    if gate:
+        if not gated or not 0 < gate < (1 << 20):
+            raise KernelError(f"gemm_int8: gate function {gate} without the gated epilogue")
+        epilogue = int(epilogue) | (int(gate) << 8)  # the kernels take it apart again and refuse what they do not have
     bias_code = _vector_code(bias, N, "gemm_int8 bias") if bias is not None else F32
-    if epilogue == EPI_ADD and (out is None or out.dtype != torch.float32):
-        raise KernelError("gemm_int8: the accumulate epilogue needs an fp32 output to add into")
-    if out is not None:
+    if out is None:
+        if epilogue == EPI_ADD:
+            raise KernelError("gemm_int8: the accumulate epilogue needs an fp32 output to add into")
+        out_dtype = out_dtype or torch.bfloat16
+        out_code = _code(out_dtype)
+        _here(aq, a_scale, wq, w_scale, uq, u_scale, bias)
+        out = _new_rows(M, N, out_dtype, aq)
+        ldo = out.stride(0)
+    else:
+        if epilogue == EPI_ADD and out.dtype != torch.float32:
+            raise KernelError("gemm_int8: the accumulate epilogue needs an fp32 output to add into")
         if out_dtype is not None and out.dtype != out_dtype:
             raise KernelError(f"gemm_int8: output is {out.dtype}, asked for {out_dtype}")
         rows, columns, ldo = _own_rows_of(out, "gemm_int8 output")
         if rows != M or columns != N:
             raise KernelError(f"gemm_int8: output is {tuple(out.shape)}, expected {(M, N)}")
         out_code = _code(out.dtype)
-    else:
-        out_dtype = out_dtype or torch.bfloat16
-        out_code = _code(out_dtype)
-    _here(a.q, a.scale, w.q, w.scale, bias, out)
-    if gated:
-        _here(w2.q, w2.scale)
-    if out is None:
-        out = _new_rows(M, N, out_dtype, a.q)
-        ldo = out.stride(0)
+        _here(aq, a_scale, wq, w_scale, uq, u_scale, bias, out)
     if M == 0 or N == 0:
         return out
-    first, second = (w.q.data_ptr(), ldw), (w2.q.data_ptr(), ldw2) if gated else (None, 0)
-    rows = (a.q.data_ptr(), lda)
-    fits = K % 16 == 0 and not (first[0] | ldw) % 16 and (not gated or (ldw2 == ldw and second[0] % 16 == 0))
-    kept = ()  # what is laid out anew, until the launches that read it are made
-    if not fits and -(-K // 16) * 16 <= INT8_MOST_INPUTS and _int8_lay_out_pays(-(-M // 64), N, K, gated):
-        first, *kept = _int8_laid_out(w.q, N, K, ldw)
+    first, second, rows = wq.data_ptr(), uq.data_ptr() if gated else None, aq.data_ptr()
+    # what the fast kernels ask of the weights; whatever else does not fit them is laid out anew, or goes to the general kernel
+    if not (K | ldw | first) % 16 and (not gated or (ldu == ldw and not second % 16)):
+        plans = _int8_plans(M, N, K, gated)
+        if (rows | lda) % 16:
+            aq, rows, lda = _int8_laid_out(aq, M, K, lda)
+    elif -(-K // 16) * 16 <= INT8_MOST_INPUTS and _int8_lay_out_pays(-(-M // 64), N, K, gated):
+        aq, rows, lda = _int8_laid_out(aq, M, K, lda)
         if gated:
-            second, *more = _int8_laid_out(w2.q, N, K, ldw2)
-            kept += more
-        rows, *more = _int8_laid_out(a.q, M, K, lda)
-        kept += more
-        K, fits = first[1], True
-    elif fits and (rows[0] | lda) % 16:
-        rows, *kept = _int8_laid_out(a.q, M, K, lda)
-    # (the kernels take the epilogue and the gate apart again and refuse what they do not have)
-    head = (*rows, a.scale.data_ptr(), *first, w.scale.data_ptr(), *second, w2.scale.data_ptr() if gated else None,
-            bias.data_ptr() if bias is not None else None, bias_code, out.data_ptr(), out_code, ldo, M, N, K, epilogue | gate << 8, gate_limit)
-    for _, kernel, size, parts in _int8_plans(M, N, K, gated) if fits else ():
-        sums = _int8_sums(M, N, gated, parts, out)
+            uq, second, ldu = _int8_laid_out(uq, N, K, ldu)
+        wq, first, ldw = _int8_laid_out(wq, N, K, ldw)
+        K = ldw
+        plans = _int8_plans(M, N, K, gated)
+    else:
+        plans = ()
+    head = (rows, lda, a_scale.data_ptr(), first, ldw, w_scale.data_ptr(), second, ldu, u_scale.data_ptr() if gated else None,
+            bias.data_ptr() if bias is not None else None, bias_code, out.data_ptr(), out_code, ldo, M, N, K, epilogue, gate_limit)
+    for _, kernel, size, parts in plans:
+        sums = _int8_sums(M, N, gated, parts, out) if parts > 1 else None
         if _try(kernel, *head, size, parts, None if sums is None else sums.data_ptr(), _stream()):
             return out
     _count("general", "jllm_gemm_int8")
     _, parts = _int8_general(-(-M // 64), N, K, gated)
-    sums = _int8_sums(M, N, gated, parts, out)
+    sums = _int8_sums(M, N, gated, parts, out) if parts > 1 else None
     _call("jllm_gemm_int8", *head, parts, None if sums is None else sums.data_ptr(), _stream())
     return out
 
 
-def _int8_sums(M: int, N: int, gated: bool, parts: int, out: torch.Tensor) -> Optional[torch.Tensor]:
+def _int8_sums(M: int, N: int, gated: bool, parts: int, out: torch.Tensor) -> torch.Tensor:
     """Where the parts of a cut K leave their sums, of this product alone."""
-    return torch.empty((parts * M * N * (2 if gated else 1),), dtype=torch.int32, device=out.device) if parts > 1 else None
+    return torch.empty((parts * M * N * (2 if gated else 1),), dtype=torch.int32, device=out.device)
 
 
 def _int8_laid_out(q: torch.Tensor, n: int, width: int, distance: int):
-    """((address, entries between rows), tensor): the rows as the fast kernels take them, with zeros up to a multiple of 16."""
+    """(tensor, its address, entries between rows): the rows as the fast kernels take them, with zeros up to a multiple of 16."""
     padded = -(-width // 16) * 16
     new = torch.empty((n, padded), dtype=torch.int8, device=q.device)
     _call("jllm_int8_lay_out", q.data_ptr(), distance, new.data_ptr(), padded, n, width, _stream())
-    return (new.data_ptr(), padded), new
+    return new, new.data_ptr(), padded
 
 
 INT8_STREAM_MOST_ROWS = 64  # of activations that the weight-streaming kernel takes

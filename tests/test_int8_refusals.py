@@ -5,8 +5,8 @@ import torch
 from jllm_serve_amd.kernels import ops
 
 
-def rows(n=4, width=32, dtype=torch.int8, scales=None):
-    return ops.Int8Rows(torch.zeros((n, width), dtype=dtype), torch.ones(n if scales is None else scales))
+def rows(n=4, width=32):
+    return ops.Int8Rows(torch.zeros((n, width), dtype=torch.int8), torch.ones(n))
 
 
 def refused(words, call, *args, **kw):
@@ -30,13 +30,20 @@ def test_quantize_rows():
 
 
 def test_int8_rows():
-    refused("must be int8", rows(dtype=torch.uint8).tensor, torch.float32)
-    refused("one entry per row", rows(scales=3).tensor, torch.float32)
-    refused("one entry per row", ops.Int8Rows(torch.zeros((4, 8), dtype=torch.int8), torch.ones(4, dtype=torch.float64)).tensor, torch.float32)
-    refused("one entry per row", ops.Int8Rows(torch.zeros((4, 8), dtype=torch.int8), torch.ones(4, 1)).tensor, torch.float32)
-    refused("contiguous fp32", ops.Int8Rows(torch.zeros((4, 8), dtype=torch.int8), torch.ones(8)[::2]).tensor, torch.float32)
-    refused("contiguous rows", ops.Int8Rows(torch.zeros((8, 4), dtype=torch.int8).t(), torch.ones(4)).tensor, torch.float32)
+    """What does not make 8-bit rows is refused where they are made."""
+    q = torch.zeros((4, 8), dtype=torch.int8)
+    refused("must be int8", ops.Int8Rows, q.view(torch.uint8), torch.ones(4))
+    refused("one entry per row", ops.Int8Rows, q, torch.ones(3))
+    refused("one entry per row", ops.Int8Rows, q, torch.ones(4, dtype=torch.float64))
+    refused("one entry per row", ops.Int8Rows, q, torch.ones(4, 1))
+    refused("contiguous fp32", ops.Int8Rows, q, torch.ones(8)[::2])
+    refused("contiguous rows", ops.Int8Rows, torch.zeros((8, 4), dtype=torch.int8).t(), torch.ones(4))
+    refused("contiguous rows", ops.Int8Rows, q[0], torch.ones(1))
     refused("float32 or bfloat16", rows().tensor, torch.float16)
+    with pytest.raises(AttributeError):
+        rows().q = q
+    with pytest.raises(AttributeError):
+        rows().scale = torch.ones(4)
 
 
 def test_rmsnorm_int8():
@@ -81,7 +88,6 @@ def test_gemm_int8():
     refused("contiguous rows", ops.gemm_int8, a, w, out=torch.zeros(6, 4).t())
     refused("float32 or bfloat16", ops.gemm_int8, a, w, out_dtype=torch.float16)
     refused("float32 or bfloat16", ops.gemm_int8, a, w, out=torch.zeros(4, 6).half())
-    refused("one entry per row", ops.gemm_int8, rows(4, scales=5), w)
 
 
 def test_a_single_row_may_have_any_stride():
