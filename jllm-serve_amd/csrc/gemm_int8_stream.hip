@@ -11,6 +11,12 @@
 // many weight rows as there are activation rows, or more. Where that leaves compute units without one, K is cut over
 // workgroups, and a second kernel adds the parts.
 //
+// us inside a graph over weights that no cache holds (in brackets the weights' way at the 6.2 TB/s of reading alone): 6,144 x 4,096 (4.1) at
+// 1, 8, 32 and 64 rows 7.3, 7.3, 8.4, 10.9; gated 12,288 x 4,096 (16.2) 20.9, 20.4, 22.0, 28.5; 4,096 x 12,288 (8.1) 11.1, 11.1, 14.8, 17.1, the last
+// in four parts; gated 17,408 x 5,120 (28.8) 36, 34.8, 39.2, 49.3. What is left is the launch and the first bytes (3), from some 32 rows on
+// the load pipe, and with K cut the second launch (3 to 4). Measured and not taken: eight waves (the same or slower from 8 MB of weights on; 4,096 x
+// 4,096 at one row 5.8 instead of 6.0), parts of K at few rows, one workgroup per compute unit where two fit.
+//
 // Needs K % 16 == 0 and 16-byte aligned rows; any N, up to 64 rows.
 #include "int8_mfma.h"
 #include "int8_parts.h"

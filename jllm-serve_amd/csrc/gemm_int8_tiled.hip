@@ -6,6 +6,12 @@
 // side). A stage's fragments are in registers before its multiplies begin; between these, evenly, a wave reads the next stage's into
 // a second set and asks for its share of the stage that takes the place of the one it multiplies. One barrier a stage.
 //
+// What binds is the pipe through which a compute unit fills its LDS, and where there are few stages the launch, the first bytes and the sum
+// of the parts. Two workgroups of 64 x 64 or 64 x 128 share a compute unit. us inside a graph: 128 x 6,144 x 4,096 12.3 (64 x 64), 487 22.2 (128 x
+// 128; in 64 x 64 26.1), 320 x 12,288 x 4,096 gated 55 (64 x 128; the large tiles 46), 80 x 12,288 x 4,096 gated 28.6 (128 x 128), 1,000 x 2,048 x 2,048
+// 11.3. Measured and not kept, since others were never far behind: 128 x 64, 128 x 128 by four waves in a ring of two, 128 x 256 and 256 x 128
+// here (the large tiles' forms are 1 to 2 % faster).
+//
 // K may be cut over gridDim.z: the parts leave their whole-number sums, and a second kernel adds them and makes the outputs.
 // Needs K % 16 == 0 and 16-byte aligned rows; any M and N.
 #include <type_traits>

@@ -11,13 +11,15 @@ struct Int8Args {
 };
 
 // Which tile workgroup b of rows x cols takes: workgroups b, b + 8, b + 16 .. share a die, which gets a run of neighbouring tiles, in
-// bands of four columns, row by row inside a band, so that its L2 passes on fewer operands
+// bands of eight columns, row by row inside a band, so that its L2 passes on fewer operands. us, bands of 2 / 4 / 8 / 16: 4,608 x 17,408 x 5,120
+// gated in tiles of 256 x 256 639 / 632 / 624 / 629, 8,192 rows 1,115 / 1,094 / 1,085 / 1,104; at most sizes the same.
+#define I8_BAND 8
 __device__ __forceinline__ void int8_die_tile(int b, int rows, int cols, int& row, int& col) {
   const int tiles = rows * cols, each = tiles >> 3, more = tiles & 7, die = b & 7;
   const int i = die * each + min(die, more) + (b >> 3);
-  const int band = i / (4 * rows), r = i - band * 4 * rows, width = min(4, cols - band * 4);
+  const int band = i / (I8_BAND * rows), r = i - band * I8_BAND * rows, width = min(I8_BAND, cols - band * I8_BAND);
   row = r / width;
-  col = band * 4 + r - row * width;
+  col = band * I8_BAND + r - row * width;
 }
 
 // four neighbouring sums of row m from column n on, of which `there` exist
@@ -43,7 +45,8 @@ __device__ __forceinline__ void int8_partial(const intx4 (&acc)[RM][CN], int lan
       if (row0 + i * 16 < M) int8_part_store(part, row0 + i * 16, col0 + j * 16, N - col0 - j * 16, N, acc[i][j]);
 }
 
-// The parts' sums ([part][weight][M][N]), V neighbouring outputs per thread (4, or 1 where N is no multiple of four): exact, so in any order
+// The parts' sums ([part][weight][M][N]), V neighbouring outputs per thread (4, or 1 where N is no multiple of four): exact, so in any order.
+// Bound by its bytes: three parts of 631 x 5,120 12 us (52 MB), four of 64 x 4,096 2.5 to 4.
 template <int V, bool GATED>
 __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__ partial, int parts, Int8Epilogue p) {
   constexpr int MATS = GATED ? 2 : 1;
