@@ -171,7 +171,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
       for (int c = 0; c < 4; ++c) {
         if (c >= there) continue;
         const float z = int8_output(sum[0][c], sa, p.end.scales.w[n + c], int8_bias(p.end, n + c));
-        y[c] = GATED ? gated<true>(z, int8_output(sum[MATS - 1][c], sa, p.end.scales.w2[n + c], 0.f), p.end.gate) : z;
+        y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.end.scales.w2[n + c], 0.f), p.end.gate) : z;
       }
       int8_store4(p.end, m, n, there, vec, y);
     }

@@ -48,6 +48,12 @@ __device__ __forceinline__ float int8_output(int sum, float sa, float sw, float 
   return y + b;
 }
 
+// The gate of two of them. Rows without numbers have a scale of NaN, and clamps would lose it.
+__device__ __forceinline__ float int8_gated(float z, float u, GateSpec gs) {
+  const float y = gated<true>(z, u, gs);
+  return z == z && u == u ? y : z + u;
+}
+
 // Four neighbouring outputs of row m from column n on, of which `there` exist; `vec`: the row's places from n on are 16-byte aligned (8 in bf16)
 __device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n, int there, bool vec, floatx4 v) {
   const size_t o = (size_t)m * p.ldo + n;
@@ -103,7 +109,7 @@ __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int la
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float z = int8_output(acc[i][j][c], sa, sw[j][c], bv[j][c]);
-        v[c] = GATED ? gated<true>(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa, su[j][c], 0.f), p.gate) : z;
+        v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa, su[j][c], 0.f), p.gate) : z;
       }
       return v;
     };

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     const float z = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, n + c));
-    y[c] = GATED ? gated<true>(z, int8_output(sum[MATS - 1][c], sa, p.scales.w2[n + c], 0.f), p.gate) : z;
+    y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.scales.w2[n + c], 0.f), p.gate) : z;
   }
   int8_store4(p, m, n, V, V == 4 && (p.ldo & 3) == 0 && ((uintptr_t)p.out & 15) == 0, y);
 }

@@ -386,6 +386,71 @@ def test_gate_functions(ops, gate, limit, M, N, K):
     close(got, y, tol)
 
 
+@pytest.mark.parametrize("gate,limit", [("silu", 0.0), ("gelu_tanh", 0.0), ("swish_clamped", 1.5)])
+@pytest.mark.parametrize("M", [3, 40, 90, 300])
+def test_rows_and_channels_without_numbers(ops, gate, limit, M):
+    """A row of activations with a NaN is a row of NaN behind every gate, a weight's channel a column; nothing else is."""
+    gen = seeded(M)
+    N, K = 300, 512
+    x, y, z = normal(gen, M, K), normal(gen, N, K), normal(gen, N, K)
+    x[1, 7], y[5, 0], z[290, K - 1] = float("nan"), float("inf"), float("nan")
+    a, w, w2 = (ops.quantize_rows(t) for t in (x, y, z))
+    got = ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, gate=ops.GATE_FUNCTIONS[gate], gate_limit=limit, out_dtype=torch.float32)
+    want = torch.zeros(M, N, dtype=torch.bool, device=DEV)
+    want[1], want[:, 5], want[:, 290] = True, True, True
+    assert torch.equal(torch.isnan(got), want)
+    want[:, 290] = False
+    want[1] = True
+    assert torch.equal(torch.isnan(ops.gemm_int8(a, w)), want)
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Rows, weights and outputs of more than 2^31 entries: the ends of them against the same rows alone."""
+    n, width = 70000, 32768
+    x = torch.empty((n, width), dtype=torch.bfloat16, device=DEV)
+    gen = seeded(1)
+    some = normal(gen, 500, width).bfloat16()
+    for r in range(0, n, 500):
+        x[r:r + 500] = some
+        x[r:r + 500] *= 1 + r % 3
+    ends = slice(n - 300, n)
+    rows = ops.quantize_rows(x)
+    want = ops.quantize_rows(x[ends])
+    assert torch.equal(rows.q[ends], want.q) and torch.equal(rows.scale[ends], want.scale)
+    assert torch.equal(rows.tensor(torch.bfloat16)[ends], want.tensor(torch.bfloat16))
+    # activations of 2.3 GB, and outputs as many
+    w = ops.quantize_rows(normal(gen, 200, width))
+    assert torch.equal(ops.gemm_int8(rows, w)[ends], ops.gemm_int8(want, w))
+    narrow = ops.Int8Rows(rows.q[:, :64], rows.scale)
+    wide = ops.quantize_rows(normal(gen, width, 64))
+    out = ops.gemm_int8(narrow, wide)
+    assert out.numel() > 1 << 31
+    assert torch.equal(out[ends], ops.gemm_int8(ops.Int8Rows(narrow.q[ends], narrow.scale[ends]), wide))
+    del out
+    # weights of 4.6 GB: both ends of two copies, for every kernel
+    q = torch.cat([rows.q, rows.q])
+    scale = torch.cat([rows.scale, rows.scale])
+    big = ops.Int8Rows(q, scale)
+    last = ops.Int8Rows(q[2 * n - 300:], scale[2 * n - 300:])
+    for m in (1, 40, 100, 700):
+        a = ops.quantize_rows(normal(gen, m, width))
+        got = ops.gemm_int8(a, big, out_dtype=torch.float32)
+        assert torch.equal(got[:, 2 * n - 300:], ops.gemm_int8(a, last, out_dtype=torch.float32))
+        got = ops.gemm_int8(a, big, w2=big, epilogue=ops.EPI_GATED)
+        assert torch.equal(got[:, 2 * n - 300:], ops.gemm_int8(a, last, w2=last, epilogue=ops.EPI_GATED))
+    # and as activations
+    got = ops.gemm_int8(big, w)
+    assert torch.equal(got[2 * n - 300:], ops.gemm_int8(last, w))
+    del q, big, last, rows
+    # the norm of a stream of 9 GB, the sum in place
+    h = x.float()
+    g = 1 + 0.1 * normal(gen, width)
+    before = h[ends].clone()
+    rows = ops.rmsnorm_int8(h, g, 1e-6, add=x)
+    want = ops.rmsnorm_int8(before, g, 1e-6, add=x[ends])
+    assert torch.equal(rows.q[ends], want.q) and torch.equal(rows.scale[ends], want.scale) and torch.equal(h[ends], before)
+
+
 def test_a_row_has_the_same_bits_in_any_batch(ops):
     """Whatever kernel, tile and cut the number of rows leads to, with every epilogue."""
     gen = seeded(11)
