@@ -12,10 +12,11 @@
 // workgroups, and a second kernel adds the parts.
 //
 // us inside a graph over weights that no cache holds (in brackets the weights' way at the 6.2 TB/s of reading alone): 6,144 x 4,096 (4.1) at
-// 1, 8, 32 and 64 rows 7.3, 7.3, 8.4, 10.9; gated 12,288 x 4,096 (16.2) 20.9, 20.4, 22.0, 28.5; 4,096 x 12,288 (8.1) 11.1, 11.1, 14.8, 17.1, the last
-// in four parts; gated 17,408 x 5,120 (28.8) 36, 34.8, 39.2, 49.3. What is left is the launch and the first bytes (3), from some 32 rows on
+// 1, 8, 32 and 64 rows 7.6, 7.6, 8.5, 10.8; gated 12,288 x 4,096 (16.2) 20.9, 20.7, 22.5, 25.4; 4,096 x 12,288 (8.1) 11.1, 11.0, 14.7, 17.5, the last
+// in four parts; gated 17,408 x 5,120 (28.8) 35, 34.8, 38.3, 45.0. What is left is the launch and the first bytes (3), from some 32 rows on
 // the load pipe, and with K cut the second launch (3 to 4). Measured and not taken: eight waves (the same or slower from 8 MB of weights on; 4,096 x
-// 4,096 at one row 5.8 instead of 6.0), parts of K at few rows, one workgroup per compute unit where two fit.
+// 4,096 at one row 5.8 instead of 6.0), parts of K at few rows, one workgroup per compute unit where two fit, the next block's
+// fragments read into a second set of registers while one multiplies (the same time where they fit, spills where not).
 //
 // Needs K % 16 == 0 and 16-byte aligned rows; any N, up to 64 rows.
 #include "int8_mfma.h"
@@ -39,9 +40,9 @@ __device__ __forceinline__ void i8_wait_block(int behind) {  // `behind` (< S) b
   wait_loads<0>();
 }
 
-// blocks of NI KB in a wave's ring: two workgroups share a compute unit where each still has two
+// blocks of NI KB in a wave's ring, out of all of the 160 KB: two workgroups share a compute unit where each still has two
 constexpr int i8_slots(int ni, int waves) {
-  const int shared = 79 / (waves * ni), fit = shared >= 2 ? shared : 159 / (waves * ni);
+  const int shared = 80 / (waves * ni), fit = shared >= 2 ? shared : 160 / (waves * ni);
   return fit > 6 ? 6 : fit;
 }
 
@@ -180,8 +181,8 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
 
 template <int NW, int NA, bool GATED>
 static int launch_stream8(const Stream8Args& a, dim3 grid, hipStream_t stream) {
-  // four waves where their rings hold two blocks each, else two
-  constexpr int NI = (GATED ? 2 : 1) * NW + NA, WAVES = i8_slots(NI, 4) >= 2 ? 4 : 2, S = i8_slots(NI, WAVES);
+  // as many waves, up to four, as have two blocks each in their rings
+  constexpr int NI = (GATED ? 2 : 1) * NW + NA, WAVES = i8_slots(NI, 4) >= 2 ? 4 : i8_slots(NI, 3) >= 2 ? 3 : 2, S = i8_slots(NI, WAVES);
   constexpr size_t smem = (size_t)S * WAVES * NI * 1024;
   if (!int8_allow_lds<gemm_int8_stream_kernel<NW, NA, GATED, WAVES>>((int)smem))
     JLLM_FAIL("gemm_int8_stream: cannot reserve %zu bytes of LDS", smem);

@@ -905,30 +905,33 @@ def _int8_laid_out(q: torch.Tensor, n: int, width: int, distance: int):
 INT8_STREAM_MOST_ROWS = 64  # of activations that the weight-streaming kernel takes
 INT8_STREAM_LOADS = (1, 2, 4, 6, 8)  # its loads of eight activation rows ...
 INT8_STREAM_WEIGHT_LOADS = (1, 2, 3, 4, 6, 8, 9, 10, 12)  # ... and of eight rows of each weight
-INT8_STREAM_WEIGHTS = (8, 12, 16, 20, 24, 28, 32, 40, 48, 56, 64, 72, 80, 96)  # rows of each weight to a workgroup
+INT8_STREAM_WEIGHTS = (8, 12, 16, 20, 24, 28, 32, 36, 40, 48, 56, 64, 72, 80, 96)  # rows of each weight to a workgroup
 INT8_CUTS = (1, 2, 3, 4, 6, 8)
 INT8_CUT_MIN_K = 512          # of a part
 INT8_CUT_MOST_GROUPS = 640    # workgroups of a cut product: more of them gain nothing
 # A cut of K: the second launch, and per sum of a part, of which there are few or many
-INT8_STREAM_CUT_US = (1.54, 3.0e-6)
+INT8_STREAM_CUT_US = (1.77, 2.28e-6)
 INT8_TILE_CUT_US = (2.62, 1.12e-6)
 
 
 def _int8_stream_us(M: int, N: int, K: int, weights: int, rows: int, parts: int) -> float:
     """Estimated time of a product of up to 64 rows in workgroups of ``rows`` weight rows (of each of ``weights`` weights) and K in ``parts``:
-    the bytes that the busiest compute unit's load pipe passes, 44.5 a nanosecond (an activation row counts for 0.59: the workgroups
-    of a compute unit ask for the same ones), against the weights' way from memory, and rounds of workgroups. Fitted to 2,800 times
-    of 15 products (0.6B to 32B shapes and three others) at 1 to 64 rows, inside a graph over as many weights as do not fit the caches: 10 % off on
-    average, and the cheapest by the estimate 1.4 % behind the best choice on average, 20 % at worst."""
+    the bytes that the busiest compute unit's load pipe passes, 48.8 a nanosecond (an activation row counts for 0.74, since the workgroups of
+    a compute unit ask for the same ones, a row that fills up a load of eight for 0.27; fewer than four waves take longer), against the
+    weights' way from memory, and rounds of workgroups. Fitted to 4,600 times of 19 products (0.6B to 32B shapes and others) at 1 to 64 rows,
+    inside a graph over as many weights as do not fit the caches: 7 % off on average, and the cheapest by the estimate 0.5 % behind the
+    best choice on average, 6 % at worst."""
     cus = compute_units()
-    loads = weights * next(n for n in INT8_STREAM_WEIGHT_LOADS if 8 * n >= rows) + M // 8
-    shared = 79 // (4 * loads) >= 2  # two workgroups fit a compute unit
+    eights = next(n for n in INT8_STREAM_WEIGHT_LOADS if 8 * n >= rows)
+    loads = weights * eights + M // 8  # KB of a block of 128 of K, of which a wave's ring holds two or more
+    waves = 4 if 160 // (4 * loads) >= 2 else 3 if 160 // (3 * loads) >= 2 else 2
+    shared = 80 // (waves * loads) >= 2  # two workgroups fit a compute unit
     blocks = -(-K // 128)
     each = -(-blocks // parts)
     groups = -(-N // rows) * -(-blocks // each)
-    pipe = -(-groups // cus) * (weights * -(-rows // 8) * 8 + 0.59 * M) * each * 128 / 44.5e3
-    memory = weights * N * K / 5.73e6
-    us = 3.2 + (pipe ** 2.25 + memory ** 2.25) ** (1 / 2.25) + 1.6 * (-(-groups // (2 * cus if shared else cus)) - 1)
+    pipe = -(-groups // cus) * (weights * (0.73 * rows + 0.27 * 8 * eights) + 0.74 * M) * each * 128 / 48.8e3 * (1.9 - 0.225 * waves)
+    memory = weights * N * K / 6.24e6
+    us = 3.3 + (pipe ** 2.27 + memory ** 2.27) ** (1 / 2.27) + (0.8 if shared else 3.1) * (-(-groups // (2 * cus if shared else cus)) - 1)
     return us + (INT8_STREAM_CUT_US[0] + INT8_STREAM_CUT_US[1] * parts * M * N * weights if parts > 1 else 0.0)
 
 
