@@ -664,12 +664,14 @@ class Int8Rows:
     stands for ``q[r] * scale[r]``. Activations are such rows by token, a weight [N, K] by output channel. Made by
     ``quantize_rows`` and ``rmsnorm_int8``, or from tensors at hand, which are looked over here, once, and keep their sizes from then on."""
 
-    __slots__ = ("_q", "_scale", "_sizes")
+    # those that the kernels make are one fp32 allocation (1.3 us on the host, a third of what it does beside a launch): the scales, and the
+    # rows from entry `_rows_at` on
+    __slots__ = ("_tensors", "_sizes", "_rows_at")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
         if q.dtype is not torch.int8:
             raise KernelError(f"8-bit rows must be int8, got {q.dtype}")
-        self._q, self._scale, self._sizes = q, scale, _rows_of(q, "8-bit rows")
+        self._tensors, self._sizes, self._rows_at = (q, scale), _rows_of(q, "8-bit rows"), None
         n = self._sizes[0]
         if scale.dtype is not torch.float32 or scale.dim() != 1 or scale.numel() != n or not scale.is_contiguous():
             raise KernelError(f"8-bit rows: the scales must be a contiguous fp32 tensor with one entry per row ({n}), got "
@@ -678,31 +680,42 @@ class Int8Rows:
     @classmethod
     def _new(cls, n: int, width: int, beside: torch.Tensor) -> "Int8Rows":
         rows = cls.__new__(cls)
-        rows._q = beside.new_empty_strided((n, width), (width, 1), dtype=torch.int8)
-        rows._scale = beside.new_empty_strided((n,), (1,), dtype=torch.float32)
+        rows._rows_at = at = -(-n // 4) * 4  # on 16 bytes
+        rows._tensors = (beside.new_empty_strided((at + -(-n * width // 4),), (1,), dtype=torch.float32),)
         rows._sizes = (n, width, width)
         return rows
 
+    def _addresses(self) -> Tuple[int, int]:  # of the rows, of the scales
+        if self._rows_at is None:
+            q, scale = self._tensors
+            return q.data_ptr(), scale.data_ptr()
+        at = self._tensors[0].data_ptr()
+        return at + 4 * self._rows_at, at
+
     @property
     def q(self) -> torch.Tensor:
-        return self._q
+        if self._rows_at is None:
+            return self._tensors[0]
+        n, width, _ = self._sizes
+        return self._tensors[0].view(torch.int8).as_strided((n, width), (width, 1), 4 * self._rows_at)
 
     @property
     def scale(self) -> torch.Tensor:
-        return self._scale
+        return self._tensors[1] if self._rows_at is None else self._tensors[0].as_strided((self._sizes[0],), (1,))
 
     @property
-    def shape(self):
-        return self._q.shape
+    def shape(self) -> torch.Size:
+        return torch.Size(self._sizes[:2])
 
     def tensor(self, dtype: torch.dtype) -> torch.Tensor:
         """The values that the rows stand for, rounded once to ``dtype``."""
         code = _code(dtype)
-        q, scale, (n, width, distance) = self._q, self._scale, self._sizes
-        _here(q, scale)
-        out = _new_rows(n, width, dtype, q)
+        n, width, distance = self._sizes
+        _here(*self._tensors)
+        out = _new_rows(n, width, dtype, self._tensors[0])
         if n and width:
-            _call("jllm_dequantize_rows", q.data_ptr(), distance, scale.data_ptr(), n, width, out.data_ptr(), code, out.stride(0), _stream())
+            q, scale = self._addresses()
+            _call("jllm_dequantize_rows", q, distance, scale, n, width, out.data_ptr(), code, out.stride(0), _stream())
         return out
 
 
@@ -773,7 +786,8 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     _here(x)
     rows = Int8Rows._new(n, width, x)
     if n:
-        _call("jllm_quantize_rows", x.data_ptr(), code, distance, n, width, rows._q.data_ptr(), width, rows._scale.data_ptr(), _stream())
+        q, scale = rows._addresses()
+        _call("jllm_quantize_rows", x.data_ptr(), code, distance, n, width, q, width, scale, _stream())
     return rows
 
 
@@ -808,8 +822,8 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
         _here(x, gain, add, out)
     rows = Int8Rows._new(n, width, x)
     if n:
-        _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, rows._q.data_ptr(), width,
-              rows._scale.data_ptr(), _stream())
+        q, scale = rows._addresses()
+        _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, q, width, scale, _stream())
     return rows
 
 
@@ -830,12 +844,12 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
     gated = w2 is not None
     if gated != (epilogue == EPI_GATED) or epilogue not in (EPI_STORE, EPI_ADD, EPI_GATED):
         raise KernelError("gemm_int8: the gated epilogue takes exactly two weights")
-    aq, a_scale, wq, w_scale, uq, u_scale, ldu = a._q, a._scale, w._q, w._scale, None, None, 0
+    operands, ldu = a._tensors + w._tensors, 0
     if gated:
         outputs, inputs, ldu = _int8_rows(w2, "gemm_int8 second weight")
         if outputs != N or inputs != K:
             raise KernelError("gemm_int8: the two weights of the gated epilogue must agree in shape")
-        uq, u_scale = w2._q, w2._scale
+        operands += w2._tensors
     if gate:
         if not gated or not 0 < gate < (1 << 20):
             raise KernelError(f"gemm_int8: gate function {gate} without the gated epilogue")
@@ -846,8 +860,8 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
             raise KernelError("gemm_int8: the accumulate epilogue needs an fp32 output to add into")
         out_dtype = out_dtype or torch.bfloat16
         out_code = _code(out_dtype)
-        _here(aq, a_scale, wq, w_scale, uq, u_scale, bias)
-        out = _new_rows(M, N, out_dtype, aq)
+        _here(*operands, bias)
+        out = _new_rows(M, N, out_dtype, operands[0])
         ldo = out.stride(0)
     else:
         if epilogue == EPI_ADD and out.dtype != torch.float32:
@@ -858,25 +872,26 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
         if rows != M or columns != N:
             raise KernelError(f"gemm_int8: output is {tuple(out.shape)}, expected {(M, N)}")
         out_code = _code(out.dtype)
-        _here(aq, a_scale, wq, w_scale, uq, u_scale, bias, out)
+        _here(*operands, bias, out)
     if M == 0 or N == 0:
         return out
-    first, second, rows = wq.data_ptr(), uq.data_ptr() if gated else None, aq.data_ptr()
+    (rows, a_scale), (first, w_scale), (second, u_scale) = a._addresses(), w._addresses(), w2._addresses() if gated else (None, None)
     # what the fast kernels ask of the weights; whatever else does not fit them is laid out anew, or goes to the general kernel
     if not (K | ldw | first) % 16 and (not gated or (ldu == ldw and not second % 16)):
         plans = _int8_plans(M, N, K, gated)
         if (rows | lda) % 16:
-            aq, rows, lda = _int8_laid_out(aq, M, K, lda)
+            laid_out, rows, lda = _int8_laid_out(rows, M, K, lda, out)
     elif -(-K // 16) * 16 <= INT8_MOST_INPUTS and _int8_lay_out_pays(-(-M // 64), N, K, gated):
-        aq, rows, lda = _int8_laid_out(aq, M, K, lda)
+        # (each new tensor keeps its memory until the launch that reads it is made)
+        laid_out, rows, lda = _int8_laid_out(rows, M, K, lda, out)
         if gated:
-            uq, second, ldu = _int8_laid_out(uq, N, K, ldu)
-        wq, first, ldw = _int8_laid_out(wq, N, K, ldw)
+            laid_out_2, second, ldu = _int8_laid_out(second, N, K, ldu, out)
+        laid_out_1, first, ldw = _int8_laid_out(first, N, K, ldw, out)
         K = ldw
         plans = _int8_plans(M, N, K, gated)
     else:
         plans = ()
-    head = (rows, lda, a_scale.data_ptr(), first, ldw, w_scale.data_ptr(), second, ldu, u_scale.data_ptr() if gated else None,
+    head = (rows, lda, a_scale, first, ldw, w_scale, second, ldu, u_scale,
             bias.data_ptr() if bias is not None else None, bias_code, out.data_ptr(), out_code, ldo, M, N, K, epilogue, gate_limit)
     for _, kernel, size, parts in plans:
         sums = _int8_sums(M, N, gated, parts, out) if parts > 1 else None
@@ -894,11 +909,11 @@ def _int8_sums(M: int, N: int, gated: bool, parts: int, out: torch.Tensor) -> to
     return torch.empty((parts * M * N * (2 if gated else 1),), dtype=torch.int32, device=out.device)
 
 
-def _int8_laid_out(q: torch.Tensor, n: int, width: int, distance: int):
-    """(tensor, its address, entries between rows): the rows as the fast kernels take them, with zeros up to a multiple of 16."""
+def _int8_laid_out(address: int, n: int, width: int, distance: int, beside: torch.Tensor):
+    """(tensor, its address, entries between rows): the rows at ``address`` as the fast kernels take them, with zeros up to a multiple of 16."""
     padded = -(-width // 16) * 16
-    new = torch.empty((n, padded), dtype=torch.int8, device=q.device)
-    _call("jllm_int8_lay_out", q.data_ptr(), distance, new.data_ptr(), padded, n, width, _stream())
+    new = torch.empty((n, padded), dtype=torch.int8, device=beside.device)
+    _call("jllm_int8_lay_out", address, distance, new.data_ptr(), padded, n, width, _stream())
     return new, new.data_ptr(), padded
 
 

@@ -94,3 +94,19 @@ def test_a_single_row_may_have_any_stride():
     """A row alone has no distance to the next: it is not refused for the stride it happens to have."""
     assert ops._own_rows_of(torch.zeros(8, 1).t(), "row") == (1, 8, 8)
     refused("2^31", ops._rows_of, torch.empty_strided((2, 1), (1 << 31, 1), dtype=torch.int8, device="meta"), "rows")
+
+
+@pytest.mark.parametrize("n, width", [(0, 5), (1, 1), (1, 16), (3, 7), (4, 8), (5, 13), (64, 129)])
+def test_rows_and_scales_of_one_allocation(n, width):
+    """What the kernels make: the scales and the rows, each on 16 bytes, neither over the other, both inside the allocation."""
+    rows = ops.Int8Rows._new(n, width, torch.empty(0))
+    assert rows.q.dtype is torch.int8 and rows.q.shape == (n, width) == rows.shape and rows.q.is_contiguous()
+    assert rows.scale.dtype is torch.float32 and rows.scale.shape == (n,) and rows.scale.is_contiguous()
+    if n:
+        assert (rows.q.data_ptr(), rows.scale.data_ptr()) == rows._addresses()
+        assert (rows.q.data_ptr() - rows.scale.data_ptr()) % 16 == 0
+        rows.q.fill_(-7)
+        rows.scale.copy_(torch.arange(n))
+        assert (rows.q == -7).all() and (rows.scale == torch.arange(n)).all()
+        storage = rows.scale.untyped_storage()
+        assert rows.q.data_ptr() + n * width <= storage.data_ptr() + storage.nbytes()
