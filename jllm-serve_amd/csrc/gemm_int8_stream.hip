@@ -148,7 +148,6 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
 #pragma unroll
       for (int m = 0; m < MT; ++m) red[wave][u][t][m][lane] = acc[u][t][m];
   __syncthreads();
-  const bool vec = (p.end.ldo & 3) == 0 && ((uintptr_t)p.end.out & 15) == 0 && (p.rows & 3) == 0;
   for (int item = threadIdx.x; item < CT * MT * 64; item += WAVES * 64) {
     const int t = item / (MT * 64), mt = item / 64 % MT;
     const int m = mt * 16 + (item & 15), in = t * 16 + (item >> 4 & 3) * 4, n = n0 + in;
@@ -174,7 +173,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
         const float z = int8_output(sum[0][c], sa, p.end.scales.w[n + c], int8_bias(p.end, n + c));
         y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.end.scales.w2[n + c], 0.f), p.end.gate) : z;
       }
-      int8_store4(p.end, m, n, there, vec, y);
+      int8_store4(p.end, m, n, there, y);
     }
   }
 }

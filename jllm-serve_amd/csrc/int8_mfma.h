@@ -54,17 +54,21 @@ __device__ __forceinline__ float int8_gated(float z, float u, GateSpec gs) {
   return z == z && u == u ? y : z + u;
 }
 
-// Four neighbouring outputs of row m from column n on, of which `there` exist; `vec`: the row's places from n on are 16-byte aligned (8 in bf16)
-__device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n, int there, bool vec, floatx4 v) {
+// Four neighbouring outputs of row m from column n on, of which `there` exist. All four are one access wherever the row begins (the
+// hardware takes it at any element).
+__device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n, int there, floatx4 v) {
   const size_t o = (size_t)m * p.ldo + n;
-  if (there == 4 && vec) {
+  if (there == 4) {
     if (p.epilogue == 1) {
-      floatx4* to = (floatx4*)((float*)p.out + o);
-      *to = *to + v;
+      floatx4 was;
+      __builtin_memcpy(&was, (float*)p.out + o, 16);
+      v += was;
+      __builtin_memcpy((float*)p.out + o, &v, 16);
     } else if (p.out_dtype == JLLM_BF16) {
-      *(u32x2*)((bf16_t*)p.out + o) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+      const u32x2 w{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+      __builtin_memcpy((bf16_t*)p.out + o, &w, 8);
     } else {
-      *(floatx4*)((float*)p.out + o) = v;
+      __builtin_memcpy((float*)p.out + o, &v, 16);
     }
     return;
   }
@@ -96,10 +100,9 @@ __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int la
       su[j][c] = GATED ? p.scales.w2[n] : 0.f;
       bv[j][c] = int8_bias(p, n);
     }
-  const bool vec = (p.ldo & 3) == 0 && ((uintptr_t)p.out & 15) == 0;
   const bool whole = n0 + (wn + 1) * NI * 16 <= p.N;  // the wave's columns are all there
   // in bf16 two neighbouring runs exchange halves between lanes first, so that a lane stores eight columns
-  const bool eights = NI % 2 == 0 && whole && vec && (p.ldo & 7) == 0 && p.epilogue != 1 && p.out_dtype == JLLM_BF16;
+  const bool eights = NI % 2 == 0 && whole && p.epilogue != 1 && p.out_dtype == JLLM_BF16;
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
     const int m = row0 + i * 16;
@@ -121,13 +124,14 @@ __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int la
         const u32x2 lo = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])}, hi = {pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3])};
         const auto a = __builtin_amdgcn_permlane16_swap(lo.x, hi.x, false, false);
         const auto b = __builtin_amdgcn_permlane16_swap(lo.y, hi.y, false, false);
-        *(u32x4*)((bf16_t*)p.out + (size_t)m * p.ldo + col0 + j * 16 - group * 4 + (group & 1) * 16 + (group >> 1) * 8) = u32x4{a[0], b[0], a[1], b[1]};
+        const u32x4 w4{a[0], b[0], a[1], b[1]};
+        __builtin_memcpy((bf16_t*)p.out + (size_t)m * p.ldo + col0 + j * 16 - group * 4 + (group & 1) * 16 + (group >> 1) * 8, &w4, 16);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         const int n = col0 + j * 16;
-        if (n < p.N) int8_store4(p, m, n, min(4, p.N - n), vec, outputs(j));
+        if (n < p.N) int8_store4(p, m, n, min(4, p.N - n), outputs(j));
       }
     }
   }

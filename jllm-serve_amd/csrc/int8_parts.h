@@ -25,8 +25,8 @@ __device__ __forceinline__ void int8_die_tile(int b, int rows, int cols, int& ro
 // four neighbouring sums of row m from column n on, of which `there` exist
 __device__ __forceinline__ void int8_part_store(int* __restrict__ part, int m, int n, int there, int N, intx4 v) {
   int* to = part + (size_t)m * N + n;
-  if (there >= 4 && ((N | n) & 3) == 0) {
-    *(intx4*)to = v;
+  if (there >= 4) {
+    __builtin_memcpy(to, &v, 16);
   } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
     const float z = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, n + c));
     y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.scales.w2[n + c], 0.f), p.gate) : z;
   }
-  int8_store4(p, m, n, V, V == 4 && (p.ldo & 3) == 0 && ((uintptr_t)p.out & 15) == 0, y);
+  int8_store4(p, m, n, V, y);
 }
 
 static inline int int8_add_parts(const int* partial, int parts, const Int8Epilogue& end, bool gated, hipStream_t stream) {
