@@ -117,15 +117,7 @@ __global__ __launch_bounds__(256) void gemm_int8_kernel(Gemm8Args p) {
   if (t + 1 < stages) stage(std::integral_constant<int, 1>{}, t + 1);
   if (t + 2 < stages) stage(std::integral_constant<int, 2>{}, t + 2);
   if (gridDim.z > 1) {
-    if constexpr (GATED) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        intx4 one[2][1] = {{acc[0][u]}, {acc[1][u]}};
-        int8_partial(one, lane, wm, wn, m0, n0, p.partial + ((size_t)blockIdx.z * 2 + u) * M * N, M, N);
-      }
-    } else {
-      int8_partial(acc, lane, wm, wn, m0, n0, p.partial + (size_t)blockIdx.z * M * N, M, N);
-    }
+    int8_partial<GATED>(acc, lane, wm, wn, m0, n0, p.partial, M, N);
     return;
   }
   int8_epilogue<GATED, 2, 2>(acc, lane, wm, wn, m0, n0, p.end);

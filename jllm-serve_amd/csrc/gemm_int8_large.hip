@@ -200,8 +200,8 @@ __global__ __launch_bounds__(L8_WAVES * 64) void gemm_int8_large_kernel(Int8Args
   constexpr int TBM = WGM * FM * 32, TBN = L8_WAVES / WGM * 64;
   const int m0 = row * TBM, n0 = col * (GATED ? TBN / 2 : TBN);
   int8_large_tile<GATED, FM, WGM>(p.A, p.lda, p.W, p.W2, p.ldw, p.end.M, p.end.N, p.K, m0, n0, [&](auto& acc, int lane, int wm, int wn) {
-    if (!GATED && gridDim.z > 1)
-      int8_partial(acc, lane, wm, wn, m0, n0, p.partial + (size_t)blockIdx.z * p.end.M * p.end.N, p.end.M, p.end.N);
+    if (gridDim.z > 1)
+      int8_partial<GATED>(acc, lane, wm, wn, m0, n0, p.partial, p.end.M, p.end.N);
     else
       int8_epilogue<GATED, 2 * FM, 4>(acc, lane, wm, wn, m0, n0, p.end);
   });
@@ -223,8 +223,8 @@ static int launch_int8_large(const Int8Args& a, int parts, hipStream_t stream) {
   return 0;
 }
 
-// `tile`: rows * 1000 + columns of the output tile (gated: twice its outputs). `parts` > 1 cuts K into so many, in whole stages of 128 (not with
-// the gated epilogue); `partial` then holds parts * M * N ints. Returns 0 when it ran, 1 when the shape is not one it takes, -1 on errors.
+// `tile`: rows * 1000 + columns of the output tile (gated: twice its outputs). `parts` > 1 cuts K into so many, in whole stages of 128;
+// `partial` then holds parts * (1 or, gated, 2) * M * N ints. Returns 0 when it ran, 1 when the shape is not one it takes, -1 on errors.
 extern "C" int jllm_gemm_int8_large(const void* A, int lda, const float* a_scale, const void* W, int ldw, const float* w_scale, const void* W2, int ldw2,
                                     const float* w2_scale, const void* bias, int bias_dtype, void* out, int out_dtype, int ldo, int M, int N, int K,
                                     int epilogue, float gate_limit, int tile, int parts, int* partial, hipStream_t stream) {
@@ -239,7 +239,7 @@ extern "C" int jllm_gemm_int8_large(const void* A, int lda, const float* a_scale
   if ((unsigned long long)M * (unsigned)lda >= (1ull << 32) || (unsigned long long)N * (unsigned)ldw >= (1ull << 32)) return 1;
   const int stages = (K + 127) / 128;
   if (parts < 1) parts = 1;
-  if (parts > 1 && (W2 || !partial || ((uintptr_t)partial & 15))) JLLM_FAIL("gemm_int8_large: %d parts of K are not possible here", parts);
+  if (parts > 1 && (!partial || ((uintptr_t)partial & 15))) JLLM_FAIL("gemm_int8_large: %d parts of K need a buffer for their sums", parts);
   if (parts > 65535 || (parts > 1 && stages <= (stages + parts - 1) / parts * (parts - 1))) return 1;  // a part without any
   const Int8Args a{(const signed char*)A, (const signed char*)W, (const signed char*)W2, partial, lda, ldw, K,
                    {{a_scale, w_scale, w2_scale}, bias, out, bias_dtype, out_dtype, ldo, M, N, epilogue, gs}};
@@ -253,5 +253,5 @@ extern "C" int jllm_gemm_int8_large(const void* A, int lda, const float* a_scale
   }
   if (rc != 0) return rc;
   JLLM_CHECK_LAUNCH("gemm_int8_large");
-  return parts > 1 ? int8_add_parts(partial, parts, a.end, false, stream) : 0;
+  return parts > 1 ? int8_add_parts(partial, parts, a.end, W2 != nullptr, stream) : 0;
 }

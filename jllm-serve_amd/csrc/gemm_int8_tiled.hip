@@ -158,8 +158,8 @@ __global__ __launch_bounds__(WGM* WGN * 64) void gemm_int8_tiled_kernel(Int8Args
     stage(std::integral_constant<int, 0>{}, std::false_type{}, t);
     if (t + 1 < nk) stage(std::integral_constant<int, 1>{}, std::false_type{}, t + 1);
   }
-  if (!GATED && gridDim.z > 1)
-    int8_partial(acc, lane, wm, wn, m0, n0, p.partial + (size_t)blockIdx.z * M * N, M, N);
+  if (gridDim.z > 1)
+    int8_partial<GATED>(acc, lane, wm, wn, m0, n0, p.partial, M, N);
   else
     int8_epilogue<GATED, RM, CN>(acc, lane, wm, wn, m0, n0, p.end);
 }
@@ -176,8 +176,8 @@ static int launch_int8_tiled(const Int8Args& a, int parts, hipStream_t stream) {
   return 0;
 }
 
-// `tile`: rows * 1000 + columns of the output tile (gated: twice its outputs). `parts` > 1 cuts K into so many, in whole stages of 128 (not with
-// the gated epilogue); `partial` then holds parts * M * N ints. Returns 0 when it ran, 1 when the shape is not one it takes, -1 on errors.
+// `tile`: rows * 1000 + columns of the output tile (gated: twice its outputs). `parts` > 1 cuts K into so many, in whole stages of 128;
+// `partial` then holds parts * (1 or, gated, 2) * M * N ints. Returns 0 when it ran, 1 when the shape is not one it takes, -1 on errors.
 extern "C" int jllm_gemm_int8_tiled(const void* A, int lda, const float* a_scale, const void* W, int ldw, const float* w_scale, const void* W2, int ldw2,
                                     const float* w2_scale, const void* bias, int bias_dtype, void* out, int out_dtype, int ldo, int M, int N, int K,
                                     int epilogue, float gate_limit, int tile, int parts, int* partial, hipStream_t stream) {
@@ -192,13 +192,13 @@ extern "C" int jllm_gemm_int8_tiled(const void* A, int lda, const float* a_scale
   if ((unsigned)lda >= (1u << 24) || (unsigned)ldw >= (1u << 24)) return 1;
   const int stages = (K + 127) / 128;
   if (parts < 1) parts = 1;
-  if (parts > 1 && (W2 || !partial || ((uintptr_t)partial & 15))) JLLM_FAIL("gemm_int8_tiled: %d parts of K are not possible here", parts);
+  if (parts > 1 && (!partial || ((uintptr_t)partial & 15))) JLLM_FAIL("gemm_int8_tiled: %d parts of K need a buffer for their sums", parts);
   if (parts > 65535 || (parts > 1 && stages <= (stages + parts - 1) / parts * (parts - 1))) return 1;  // a part without any
   const Int8Args a{(const signed char*)A, (const signed char*)W, (const signed char*)W2, partial, lda, ldw, K,
                    {{a_scale, w_scale, w2_scale}, bias, out, bias_dtype, out_dtype, ldo, M, N, epilogue, gs}};
   int rc;
 #define T8_CASE(CODE, ...) \
-  case CODE: rc = W2 ? launch_int8_tiled<true, __VA_ARGS__>(a, 1, stream) : launch_int8_tiled<false, __VA_ARGS__>(a, parts, stream); break;
+  case CODE: rc = W2 ? launch_int8_tiled<true, __VA_ARGS__>(a, parts, stream) : launch_int8_tiled<false, __VA_ARGS__>(a, parts, stream); break;
   switch (tile) {
     T8_CASE(64064, 2, 2, 2, 2, 4)
     T8_CASE(64128, 2, 4, 2, 2, 3)
@@ -208,5 +208,5 @@ extern "C" int jllm_gemm_int8_tiled(const void* A, int lda, const float* a_scale
 #undef T8_CASE
   if (rc != 0) return rc;
   JLLM_CHECK_LAUNCH("gemm_int8_tiled");
-  return parts > 1 ? int8_add_parts(partial, parts, a.end, false, stream) : 0;
+  return parts > 1 ? int8_add_parts(partial, parts, a.end, W2 != nullptr, stream) : 0;
 }

@@ -5,7 +5,7 @@
 // what the tiled kernels take
 struct Int8Args {
   const signed char *A, *W, *W2;
-  int* partial;  // [part][M][N]
+  int* partial;  // [part][weight][M][N]
   int lda, ldw, K;
   Int8Epilogue end;
 };
@@ -34,15 +34,20 @@ __device__ __forceinline__ void int8_part_store(int* __restrict__ part, int m, i
   }
 }
 
-// A wave's sums as its part of a cut K
-template <int RM, int CN>
-__device__ __forceinline__ void int8_partial(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, int* part, int M, int N) {
-  const int row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * CN * 16 + lane / 16 * 4;
+// A wave's sums (as `int8_epilogue` has them) as its part blockIdx.z of a cut K
+template <bool GATED, int RM, int CN>
+__device__ __forceinline__ void int8_partial(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, int* partial, int M, int N) {
+  constexpr int NI = GATED ? CN / 2 : CN;
+  const size_t all = (size_t)M * N;
+  int* part = partial + blockIdx.z * all * (GATED ? 2 : 1);
+  const int row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * NI * 16 + lane / 16 * 4;
 #pragma unroll
   for (int i = 0; i < RM; ++i)
 #pragma unroll
-    for (int j = 0; j < CN; ++j)
-      if (row0 + i * 16 < M) int8_part_store(part, row0 + i * 16, col0 + j * 16, N - col0 - j * 16, N, acc[i][j]);
+    for (int j = 0; j < CN; ++j) {
+      const int n = col0 + j % NI * 16;
+      if (row0 + i * 16 < M) int8_part_store(part + j / NI * all, row0 + i * 16, n, N - n, N, acc[i][j]);
+    }
 }
 
 // The parts' sums ([part][weight][M][N]), V neighbouring outputs per thread (4, or 1 where N is no multiple of four): exact, so in any order.

@@ -963,7 +963,7 @@ def _int8_tile_us(tile: int, M: int, N: int, K: int, weights: int, parts: int) -
     """The product in tiles of one kind with K in ``parts``: rounds of workgroups, one or two to a compute unit, against the weights' way from
     memory. Fitted to 3,500 times of 14 products at 80 to 4,096 rows, taken as for `_int8_stream_us`: 8 % off on average, the cheapest by
     the estimate 0.5 % behind the best choice on average, 10 % at worst (without the tiles of 64 x 64 9 %, without either of the others 1 to 2 %
-    on average)."""
+    on average). Gated products in parts, 1,800 times of ten products at 80 to 1,024 rows: 1.1 % behind on average, 14 % at worst."""
     cus = compute_units()
     rows, columns = divmod(tile, 1000)
     fixed, lone, more, round_us, *pair = INT8_TILE_US[tile]
@@ -976,7 +976,7 @@ def _int8_tile_us(tile: int, M: int, N: int, K: int, weights: int, parts: int) -
     elif rest:
         us += stages * (lone + more * rest / cus) + round_us
     us = fixed + math.hypot(us, weights * N * K / INT8_TILE_BYTES_PER_US)
-    return us + (INT8_TILE_CUT_US[0] + INT8_TILE_CUT_US[1] * parts * M * N if parts > 1 else 0.0)
+    return us + (INT8_TILE_CUT_US[0] + INT8_TILE_CUT_US[1] * parts * M * N * (2.4 if weights == 2 else 1) if parts > 1 else 0.0)
 
 
 @functools.lru_cache(maxsize=8192)
@@ -1000,7 +1000,7 @@ def _int8_choices(units: int, N: int, K: int, gated: bool):
         if large and K <= 128:
             continue
         found.append(min((_int8_tile_us(tile, units, N, K, weights, parts), tile, parts) for tile in INT8_TILE_US if (tile >= INT8_LARGE_FROM) == large
-                         for parts in cuts(-(-N // (tile % 1000 // weights)) * -(-units // (tile // 1000)), (1,) if gated else INT8_CUTS)))
+                         for parts in cuts(-(-N // (tile % 1000 // weights)) * -(-units // (tile // 1000)))))
     found.sort()
     # (the large tiles decline operands of 4 GB: then the others' best)
     return tuple((us, "jllm_gemm_int8_large" if tile >= INT8_LARGE_FROM else "jllm_gemm_int8_tiled", tile, parts) for us, tile, parts in found)

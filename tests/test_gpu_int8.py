@@ -346,6 +346,51 @@ def test_every_tile(ops, monkeypatch, kernel, tile, K):
                 assert torch.equal(ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, out_dtype=torch.float32), gated)
 
 
+@pytest.mark.parametrize("kernel,tile", TILES)
+@pytest.mark.parametrize("K", [144, 256, 656, 1040, 2192])
+def test_every_tile_gated_in_parts(ops, monkeypatch, kernel, tile, K):
+    """Both weights' sums of every part, rows and columns ending inside a tile: the bits of the general kernel."""
+    gen = seeded(tile + K + 1)
+    for M, N in ((1, 5), (70, 300), (300, 130), (513, 523)):
+        a, w, w2 = operands(ops, gen, M, N, K)
+        bias = normal(gen, N)
+        call = lambda dtype: ops.gemm_int8(a, w, w2=w2, bias=bias, epilogue=ops.EPI_GATED, out_dtype=dtype)
+        monkeypatch.setattr(ops, "_int8_plans", lambda *args: ())
+        want, narrow = call(torch.float32), call(torch.bfloat16)
+        for parts in (2, 3, 5):
+            stages = -(-K // 128)
+            if stages <= -(-stages // parts) * (parts - 1):
+                continue
+            monkeypatch.setattr(ops, "_int8_plans", lambda *args: ((0.0, kernel, tile, parts),))
+            ops.reset_stats()
+            assert torch.equal(call(torch.float32), want) and torch.equal(call(torch.bfloat16), narrow)
+            assert ops.stats()["ran"] == {kernel: 2}
+
+
+PLACES = [("", 0, 1)] + [(kernel, tile, parts) for kernel, tile in TILES + [("jllm_gemm_int8_stream", 24)] for parts in (1, 2)]
+
+
+@pytest.mark.parametrize("kernel,size,parts", PLACES)
+def test_outputs_at_any_element(ops, monkeypatch, kernel, size, parts):
+    """Rows of outputs that begin at any element and lie any distance apart, whole runs of columns and cut ones: the values, and nothing beside them."""
+    gen = seeded(size + parts)
+    M, K = 64 if kernel.endswith("stream") else 150, 656
+    for N, pad, at in ((261, 0, 1), (256, 1, 0), (256, 3, 5), (262, 2, 2), (512, 5, 3)):
+        a, w, w2 = operands(ops, gen, M, N, K)
+        for dtype in (torch.float32, torch.bfloat16):
+            for kw in (dict(), dict(w2=w2, epilogue=ops.EPI_GATED)) + ((dict(epilogue=ops.EPI_ADD),) if dtype == torch.float32 else ()):
+                adds = kw.get("epilogue") == ops.EPI_ADD
+                monkeypatch.setattr(ops, "_int8_plans", lambda *args: ())
+                want = ops.gemm_int8(a, w, out=torch.ones(M, N, device="cuda"), **kw) if adds else ops.gemm_int8(a, w, out_dtype=dtype, **kw)
+                monkeypatch.setattr(ops, "_int8_plans", lambda *args: ((0.0, kernel, size, parts),) if kernel else ())
+                memory = torch.ones(at + M * (N + pad) + 8, dtype=dtype, device="cuda")
+                out = memory[at:at + M * (N + pad)].view(M, N + pad)[:, :N]
+                ops.gemm_int8(a, w, out=out, **kw)
+                assert torch.equal(out, want)
+                out.fill_(1)
+                assert (memory == 1).all()
+
+
 @pytest.mark.parametrize("M", [1, 8, 9, 30, 48, 64])
 @pytest.mark.parametrize("K", [16, 128, 144, 1040, 2176, 8208])
 def test_every_number_of_weight_rows(ops, monkeypatch, M, K):
