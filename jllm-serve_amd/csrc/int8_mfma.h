@@ -51,7 +51,7 @@ __device__ __forceinline__ float int8_output(int sum, float sa, float sw, float 
 // The gate of two of them. Rows without numbers have a scale of NaN, and clamps would lose it.
 __device__ __forceinline__ float int8_gated(float z, float u, GateSpec gs) {
   const float y = gated<true>(z, u, gs);
-  return z == z && u == u ? y : z + u;
+  return gs.fn != JLLM_GATE_SWISH_CLAMPED || (z == z && u == u) ? y : z + u;
 }
 
 // Four neighbouring outputs of row m from column n on, of which `there` exist. All four are one access wherever the row begins (the
@@ -86,8 +86,8 @@ __device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n,
 
 // A wave's accumulators, CN runs of four columns for each of its RM blocks of 16 rows (gated: [.][j] and [.][j + CN / 2] are the two weights' of the
 // same outputs), row block by row block, so that hardly more than the sums themselves is in registers.
-template <bool GATED, int RM, int CN>
-__device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
+template <bool GATED, int FN, int RM, int CN>
+__device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
   constexpr int NI = GATED ? CN / 2 : CN;
   const int group = lane / 16, row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * NI * 16 + group * 4;
   float sw[NI][4], su[NI][4], bv[NI][4];
@@ -112,7 +112,7 @@ __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int la
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float z = int8_output(acc[i][j][c], sa, sw[j][c], bv[j][c]);
-        v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa, su[j][c], 0.f), p.gate) : z;
+        v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa, su[j][c], 0.f), GateSpec{FN, p.gate.limit}) : z;
       }
       return v;
     };
@@ -135,6 +135,17 @@ __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int la
       }
     }
   }
+}
+
+// The same, each gate function in code of its own: chosen output by output it took as long as the gates themselves
+template <bool GATED, int RM, int CN>
+__device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
+  if (!GATED || p.gate.fn == JLLM_GATE_SILU)
+    int8_outputs<GATED, JLLM_GATE_SILU>(acc, lane, wm, wn, m0, n0, p);
+  else if (p.gate.fn == JLLM_GATE_GELU_TANH)
+    int8_outputs<GATED, JLLM_GATE_GELU_TANH>(acc, lane, wm, wn, m0, n0, p);
+  else
+    int8_outputs<GATED, JLLM_GATE_SWISH_CLAMPED>(acc, lane, wm, wn, m0, n0, p);
 }
 
 // Above 64 KB a kernel's dynamic LDS has to be allowed first, on every device once

@@ -432,6 +432,20 @@ def test_gate_functions(ops, gate, limit, M, N, K):
 
 
 @pytest.mark.parametrize("gate,limit", [("silu", 0.0), ("gelu_tanh", 0.0), ("swish_clamped", 1.5)])
+def test_gate_functions_alike_in_every_kernel(ops, monkeypatch, gate, limit):
+    gen = seeded(31)
+    for kernel, size in TILES + [("jllm_gemm_int8_stream", 24)]:
+        M, N, K = 64 if kernel.endswith("stream") else 300, 264, 1040
+        a, w, w2 = operands(ops, gen, M, N, K)
+        call = lambda: ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, gate=ops.GATE_FUNCTIONS[gate], gate_limit=limit, out_dtype=torch.float32)
+        monkeypatch.setattr(ops, "_int8_plans", lambda *args: ())
+        want = call()
+        for parts in (1, 3):
+            monkeypatch.setattr(ops, "_int8_plans", lambda *args: ((0.0, kernel, size, parts),))
+            assert torch.equal(call(), want), (kernel, size, parts)
+
+
+@pytest.mark.parametrize("gate,limit", [("silu", 0.0), ("gelu_tanh", 0.0), ("swish_clamped", 1.5)])
 @pytest.mark.parametrize("M", [3, 40, 90, 300])
 def test_rows_and_channels_without_numbers(ops, gate, limit, M):
     """A row of activations with a NaN is a row of NaN behind every gate, a weight's channel a column; nothing else is."""
