@@ -84,54 +84,119 @@ __device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n,
   }
 }
 
+// The four values of a vector per column from column n on, `whole`: all of them there. Any alignment of an entry.
+__device__ __forceinline__ void int8_columns(const float* from, int n, int N, bool whole, float (&to)[4]) {
+  if (whole) {
+    __builtin_memcpy(to, from + n, 16);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) to[c] = from[min(n + c, N - 1)];
+  }
+}
+
 // A wave's accumulators, CN runs of four columns for each of its RM blocks of 16 rows (gated: [.][j] and [.][j + CN / 2] are the two weights' of the
-// same outputs), row block by row block, so that hardly more than the sums themselves is in registers.
+// same outputs), row block by row block, so that hardly more than the sums themselves is in registers. Where all of its columns are there
+// it goes without a branch per output, and everything is requested before the first output is stored (behind a store the compiler moves no
+// load forward, and each would wait for its own way); what the outputs are added to, one block of rows ahead.
 template <bool GATED, int FN, int RM, int CN>
 __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
   constexpr int NI = GATED ? CN / 2 : CN;
   const int group = lane / 16, row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * NI * 16 + group * 4;
-  float sw[NI][4], su[NI][4], bv[NI][4];
+  const bool whole = n0 + (wn + 1) * NI * 16 <= p.N;  // the same in all lanes
+  float sa[RM], sw[NI][4], su[NI][4], bv[NI][4];
 #pragma unroll
-  for (int j = 0; j < NI; ++j)
+  for (int i = 0; i < RM; ++i) sa[i] = p.scales.a[min(row0 + i * 16, p.M - 1)];
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    int8_columns(p.scales.w, col0 + j * 16, p.N, whole, sw[j]);
+    if (GATED) int8_columns(p.scales.w2, col0 + j * 16, p.N, whole, su[j]);
+  }
+  if (!p.bias) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) bv[j][c] = 0.f;
+  } else if (p.bias_dtype == JLLM_BF16) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) bv[j][c] = ldf((const bf16_t*)p.bias, min(col0 + j * 16 + c, p.N - 1));
+  } else {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) int8_columns((const float*)p.bias, col0 + j * 16, p.N, whole, bv[j]);
+  }
+  auto outputs = [&](int i, int j) {
+    floatx4 v;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int n = min(col0 + j * 16 + c, p.N - 1);
-      sw[j][c] = p.scales.w[n];
-      su[j][c] = GATED ? p.scales.w2[n] : 0.f;
-      bv[j][c] = int8_bias(p, n);
+      const float z = int8_output(acc[i][j][c], sa[i], sw[j][c], bv[j][c]);
+      v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa[i], su[j][c], 0.f), GateSpec{FN, p.gate.limit}) : z;
     }
-  const bool whole = n0 + (wn + 1) * NI * 16 <= p.N;  // the wave's columns are all there
-  // in bf16 two neighbouring runs exchange halves between lanes first, so that a lane stores eight columns
-  const bool eights = NI % 2 == 0 && whole && p.epilogue != 1 && p.out_dtype == JLLM_BF16;
+    return v;
+  };
+  if (!whole) {
 #pragma unroll
-  for (int i = 0; i < RM; ++i) {
-    const int m = row0 + i * 16;
-    const float sa = p.scales.a[min(m, p.M - 1)];
-    auto outputs = [&](int j) {
-      floatx4 v;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float z = int8_output(acc[i][j][c], sa, sw[j][c], bv[j][c]);
-        v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa, su[j][c], 0.f), GateSpec{FN, p.gate.limit}) : z;
-      }
-      return v;
-    };
-    if (m >= p.M) continue;
-    if (eights) {
-#pragma unroll
-      for (int j = 0; j < NI / 2 * 2; j += 2) {
-        const floatx4 v = outputs(j), w = outputs(j + 1);
-        const u32x2 lo = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])}, hi = {pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3])};
-        const auto a = __builtin_amdgcn_permlane16_swap(lo.x, hi.x, false, false);
-        const auto b = __builtin_amdgcn_permlane16_swap(lo.y, hi.y, false, false);
-        const u32x4 w4{a[0], b[0], a[1], b[1]};
-        __builtin_memcpy((bf16_t*)p.out + (size_t)m * p.ldo + col0 + j * 16 - group * 4 + (group & 1) * 16 + (group >> 1) * 8, &w4, 16);
-      }
-    } else {
+    for (int i = 0; i < RM; ++i) {
+      const int m = row0 + i * 16;
+      if (m >= p.M) continue;
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         const int n = col0 + j * 16;
-        if (n < p.N) int8_store4(p, m, n, min(4, p.N - n), outputs(j));
+        if (n < p.N) int8_store4(p, m, n, min(4, p.N - n), outputs(i, j));
+      }
+    }
+  } else if (!GATED && p.epilogue == 1) {
+    float* out = (float*)p.out + col0;
+    floatx4 was[2][NI];
+    auto fetch = [&](int i) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) __builtin_memcpy(&was[i & 1][j], out + (size_t)min(row0 + i * 16, p.M - 1) * p.ldo + j * 16, 16);
+    };
+    fetch(0);
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      if (i + 1 < RM) fetch(i + 1);
+      if (row0 + i * 16 >= p.M) continue;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const floatx4 v = was[i & 1][j] + outputs(i, j);
+        __builtin_memcpy(out + (size_t)(row0 + i * 16) * p.ldo + j * 16, &v, 16);
+      }
+    }
+  } else if (p.out_dtype == JLLM_BF16) {
+    bf16_t* out = (bf16_t*)p.out + col0;
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      if (row0 + i * 16 >= p.M) continue;
+      bf16_t* to = out + (size_t)(row0 + i * 16) * p.ldo;
+      if constexpr (NI % 2 == 0) {  // two neighbouring runs exchange halves between lanes first, so that a lane stores eight columns
+#pragma unroll
+        for (int j = 0; j < NI; j += 2) {
+          const floatx4 v = outputs(i, j), w = outputs(i, j + 1);
+          const u32x2 lo = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])}, hi = {pack_bf16(w[0], w[1]), pack_bf16(w[2], w[3])};
+          const auto a = __builtin_amdgcn_permlane16_swap(lo.x, hi.x, false, false);
+          const auto b = __builtin_amdgcn_permlane16_swap(lo.y, hi.y, false, false);
+          const u32x4 w4{a[0], b[0], a[1], b[1]};
+          __builtin_memcpy(to + j * 16 - group * 4 + (group & 1) * 16 + (group >> 1) * 8, &w4, 16);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          const floatx4 v = outputs(i, j);
+          const u32x2 w{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+          __builtin_memcpy(to + j * 16, &w, 8);
+        }
+      }
+    }
+  } else {
+    float* out = (float*)p.out + col0;
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      if (row0 + i * 16 >= p.M) continue;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const floatx4 v = outputs(i, j);
+        __builtin_memcpy(out + (size_t)(row0 + i * 16) * p.ldo + j * 16, &v, 16);
       }
     }
   }
