@@ -12,8 +12,8 @@
 // workgroups, and a second kernel adds the parts.
 //
 // us inside a graph over weights that no cache holds (in brackets the weights' way at the 6.2 TB/s of reading alone): 6,144 x 4,096 (4.1) at
-// 1, 8, 32 and 64 rows 7.6, 7.6, 8.5, 10.8; gated 12,288 x 4,096 (16.2) 20.9, 20.7, 22.5, 25.4; 4,096 x 12,288 (8.1) 11.1, 11.0, 14.7, 17.5, the last
-// in four parts; gated 17,408 x 5,120 (28.8) 35, 34.8, 38.3, 45.0. What is left is the launch and the first bytes (3), from some 32 rows on
+// 1, 8, 32 and 64 rows 7.0, 7.1, 8.2, 10.7; gated 12,288 x 4,096 (16.2) 20.7, 20.6, 22.2, 24.9; 4,096 x 12,288 (8.1) 11.0, 10.9, 14.5, 17.5, the last
+// in four parts; gated 17,408 x 5,120 (28.8) 35, 34.5, 38, 44.5. What is left is the launch and the first bytes (3), from some 32 rows on
 // the load pipe, and with K cut the second launch (3 to 4). Measured and not taken: eight waves (the same or slower from 8 MB of weights on; 4,096 x
 // 4,096 at one row 5.8 instead of 6.0), parts of K at few rows, one workgroup per compute unit where two fit, the next block's
 // fragments read into a second set of registers while one multiplies (the same time where they fit, spills where not).
@@ -78,6 +78,46 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
   const unsigned char* ring = smem + (size_t)wave * S * NI * 1024;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)ring;
   const int total = wave < nblk ? (nblk - wave + WAVES - 1) / WAVES : 0;
+  // ---- outputs: a thread has items of four columns of a row. What an item needs beside its sums is on its way one item ahead, the first's
+  // from here on (us, asked for behind the sums / so: 1 x 4,096 x 4,096 into the residual 5.8 / 5.15, 8 x 2,560 x 2,560 with a bias 4.5 / 3.85, 64 x 12,288 x
+  // 4,096 gated 25.6 / 24.9)
+  constexpr int ITEMS = (CT * MT + WAVES - 1) / WAVES;
+  const bool whole_k = gridDim.y == 1;
+  struct Item {
+    int m, n, there;  // there <= 0: none
+    float sa, sw[4], su[4];
+    uint32_t bias[4];  // as it was loaded: to make a number of it here would be to wait for it
+    floatx4 was;
+  };
+  auto item_of = [&](int i) {
+    const int item = threadIdx.x + i * WAVES * 64, t = item / (MT * 64), mt = item / 64 % MT, in = t * 16 + (item >> 4 & 3) * 4;
+    Item it;
+    it.m = mt * 16 + (item & 15), it.n = n0 + in;
+    it.there = item < CT * MT * 64 && it.m < M ? min(4, min(N - it.n, p.rows - in)) : 0;
+    if (whole_k && wave + i * WAVES < CT * MT) {
+      const int m = min(it.m, M - 1);
+      it.sa = p.end.scales.a[m];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int n = min(it.n + c, N - 1);
+        it.sw[c] = p.end.scales.w[n];
+        if (GATED) it.su[c] = p.end.scales.w2[n];
+        if (!GATED && p.end.epilogue == 1) it.was[c] = ((const float*)p.end.out)[(size_t)m * p.end.ldo + n];
+        it.bias[c] = 0;
+      }
+      if (p.end.bias) {
+        if (p.end.bias_dtype == JLLM_BF16) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) it.bias[c] = ((const uint16_t*)p.end.bias)[min(it.n + c, N - 1)];
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) it.bias[c] = ((const uint32_t*)p.end.bias)[min(it.n + c, N - 1)];
+        }
+      }
+    }
+    return it;
+  };
+  Item next = item_of(0);
   auto issue = [&](int i, int slot) {
     int b = wave + i * WAVES + turn;
     b = first + (b >= nblk ? b - nblk : b);
@@ -138,7 +178,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
           for (int m = 0; m < MT; ++m) acc[u][t][m] = mfma16_i8(w[u][t][j], a[m][j], acc[u][t][m]);
     if (++slot == S) slot = 0;
   }
-  // ---- the waves' sums meet in LDS; then a thread has items of four columns of a row
+  // ---- the waves' sums meet in LDS
   __syncthreads();  // every wave is done with its ring
   intx4(*red)[MATS][CT][MT][64] = (intx4(*)[MATS][CT][MT][64])smem;
 #pragma unroll
@@ -148,11 +188,12 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
 #pragma unroll
       for (int m = 0; m < MT; ++m) red[wave][u][t][m][lane] = acc[u][t][m];
   __syncthreads();
-  for (int item = threadIdx.x; item < CT * MT * 64; item += WAVES * 64) {
-    const int t = item / (MT * 64), mt = item / 64 % MT;
-    const int m = mt * 16 + (item & 15), in = t * 16 + (item >> 4 & 3) * 4, n = n0 + in;
-    const int there = min(4, min(N - n, p.rows - in));
-    if (m >= M || there <= 0) continue;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const Item it = next;
+    if (i + 1 < ITEMS) next = item_of(i + 1);
+    if (it.there <= 0) continue;
+    const int item = threadIdx.x + i * WAVES * 64, t = item / (MT * 64), mt = item / 64 % MT;
     intx4 sum[MATS];
 #pragma unroll
     for (int u = 0; u < MATS; ++u) {
@@ -160,20 +201,20 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) sum[u] += red[w][u][t][mt][item & 63];
     }
-    if (gridDim.y > 1) {
+    if (!whole_k) {
 #pragma unroll
       for (int u = 0; u < MATS; ++u)
-        int8_part_store(p.partial + ((size_t)blockIdx.y * MATS + u) * M * N, m, n, there, N, sum[u]);
+        int8_part_store(p.partial + ((size_t)blockIdx.y * MATS + u) * M * N, it.m, it.n, it.there, N, sum[u]);
     } else {
-      const float sa = p.end.scales.a[m];
-      floatx4 y{0.f, 0.f, 0.f, 0.f};
+      floatx4 y;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if (c >= there) continue;
-        const float z = int8_output(sum[0][c], sa, p.end.scales.w[n + c], int8_bias(p.end, n + c));
-        y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.end.scales.w2[n + c], 0.f), p.end.gate) : z;
+        const float b = __uint_as_float(p.end.bias_dtype == JLLM_BF16 ? it.bias[c] << 16 : it.bias[c]);
+        const float z = int8_output(sum[0][c], it.sa, it.sw[c], b);
+        y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], it.sa, it.su[c], 0.f), p.end.gate) : z;
       }
-      int8_store4(p.end, m, n, there, y);
+      if (!GATED && p.end.epilogue == 1) y += it.was;
+      int8_store4(p.end, it.m, it.n, it.there, y);
     }
   }
 }

@@ -54,17 +54,19 @@ __device__ __forceinline__ float int8_gated(float z, float u, GateSpec gs) {
   return gs.fn != JLLM_GATE_SWISH_CLAMPED || (z == z && u == u) ? y : z + u;
 }
 
-// Four neighbouring outputs of row m from column n on, of which `there` exist. All four are one access wherever the row begins (the
-// hardware takes it at any element).
+// What four neighbouring outputs of row m from column n on are added to
+__device__ __forceinline__ floatx4 int8_load4(const Int8Epilogue& p, int m, int n) {
+  floatx4 v;
+  __builtin_memcpy(&v, (const float*)p.out + (size_t)m * p.ldo + n, 16);
+  return v;
+}
+
+// Four neighbouring outputs of row m from column n on, of which `there` exist (what they are added to is in them). All four are one access
+// wherever the row begins (the hardware takes it at any element).
 __device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n, int there, floatx4 v) {
   const size_t o = (size_t)m * p.ldo + n;
   if (there == 4) {
-    if (p.epilogue == 1) {
-      floatx4 was;
-      __builtin_memcpy(&was, (float*)p.out + o, 16);
-      v += was;
-      __builtin_memcpy((float*)p.out + o, &v, 16);
-    } else if (p.out_dtype == JLLM_BF16) {
+    if (p.out_dtype == JLLM_BF16) {
       const u32x2 w{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
       __builtin_memcpy((bf16_t*)p.out + o, &w, 8);
     } else {
@@ -75,9 +77,7 @@ __device__ __forceinline__ void int8_store4(const Int8Epilogue& p, int m, int n,
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     if (c >= there) continue;
-    if (p.epilogue == 1)
-      ((float*)p.out)[o + c] += v[c];
-    else if (p.out_dtype == JLLM_BF16)
+    if (p.out_dtype == JLLM_BF16)
       stf((bf16_t*)p.out, o + c, v[c]);
     else
       stf((float*)p.out, o + c, v[c]);
@@ -142,7 +142,13 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
         const int n = col0 + j * 16;
-        if (n < p.N) int8_store4(p, m, n, min(4, p.N - n), outputs(i, j));
+        if (n >= p.N) continue;
+        floatx4 v = outputs(i, j);
+        if (!GATED && p.epilogue == 1) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] += ((const float*)p.out)[(size_t)m * p.ldo + min(n + c, p.N - 1)];
+        }
+        int8_store4(p, m, n, min(4, p.N - n), v);
       }
     }
   } else if (!GATED && p.epilogue == 1) {
@@ -150,7 +156,7 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
     floatx4 was[2][NI];
     auto fetch = [&](int i) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) __builtin_memcpy(&was[i & 1][j], out + (size_t)min(row0 + i * 16, p.M - 1) * p.ldo + j * 16, 16);
+      for (int j = 0; j < NI; ++j) was[i & 1][j] = int8_load4(p, min(row0 + i * 16, p.M - 1), col0 + j * 16);
     };
     fetch(0);
 #pragma unroll

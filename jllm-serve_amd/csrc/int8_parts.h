@@ -58,6 +58,11 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
   const size_t all = (size_t)p.M * p.N, i = ((size_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (i >= all) return;
   const int m = (int)(i / p.N), n = (int)(i - (size_t)m * p.N);
+  floatx4 y{0.f, 0.f, 0.f, 0.f}, was{0.f, 0.f, 0.f, 0.f};
+  if (!GATED && p.epilogue == 1) {  // on its way together with the sums
+    if (V == 4) was = int8_load4(p, m, n);
+    else was[0] = ((const float*)p.out)[(size_t)m * p.ldo + n];
+  }
   int sum[MATS][V] = {};
 #pragma unroll 4
   for (int z = 0; z < parts; ++z)
@@ -69,12 +74,12 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
       for (int c = 0; c < V; ++c) sum[u][c] += s[c];
     }
   const float sa = p.scales.a[m];
-  floatx4 y{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     const float z = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, n + c));
     y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.scales.w2[n + c], 0.f), p.gate) : z;
   }
+  if (!GATED && p.epilogue == 1) y += was;
   int8_store4(p, m, n, V, y);
 }
 
