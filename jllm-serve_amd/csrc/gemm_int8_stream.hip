@@ -86,7 +86,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
   struct Item {
     int m, n, there;  // there <= 0: none
     float sa, sw[4], su[4];
-    uint32_t bias[4];  // as it was loaded: to make a number of it here would be to wait for it
+    uint32_t bias[4];
     floatx4 was;
   };
   auto item_of = [&](int i) {
@@ -103,17 +103,8 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
         it.sw[c] = p.end.scales.w[n];
         if (GATED) it.su[c] = p.end.scales.w2[n];
         if (!GATED && p.end.epilogue == 1) it.was[c] = ((const float*)p.end.out)[(size_t)m * p.end.ldo + n];
-        it.bias[c] = 0;
       }
-      if (p.end.bias) {
-        if (p.end.bias_dtype == JLLM_BF16) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) it.bias[c] = ((const uint16_t*)p.end.bias)[min(it.n + c, N - 1)];
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) it.bias[c] = ((const uint32_t*)p.end.bias)[min(it.n + c, N - 1)];
-        }
-      }
+      int8_load_bias(p.end, it.n, it.bias);
     }
     return it;
   };
@@ -209,8 +200,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
       floatx4 y;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float b = __uint_as_float(p.end.bias_dtype == JLLM_BF16 ? it.bias[c] << 16 : it.bias[c]);
-        const float z = int8_output(sum[0][c], it.sa, it.sw[c], b);
+        const float z = int8_output(sum[0][c], it.sa, it.sw[c], int8_bias(p.end, it.bias[c]));
         y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], it.sa, it.su[c], 0.f), p.end.gate) : z;
       }
       if (!GATED && p.end.epilogue == 1) y += it.was;

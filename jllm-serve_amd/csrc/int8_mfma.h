@@ -36,9 +36,21 @@ struct Int8Epilogue {
   GateSpec gate;
 };
 
-__device__ __forceinline__ float int8_bias(const Int8Epilogue& p, int n) {
-  return !p.bias ? 0.f : p.bias_dtype == JLLM_BF16 ? ldf((const bf16_t*)p.bias, n) : ldf((const float*)p.bias, n);
+// The bias of C columns from n on (the last column's behind it) as it lies in memory: to make numbers of it would be to wait for it
+template <int C>
+__device__ __forceinline__ void int8_load_bias(const Int8Epilogue& p, int n, uint32_t (&raw)[C]) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) raw[c] = 0;
+  if (!p.bias) return;
+  if (p.bias_dtype == JLLM_BF16) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) raw[c] = ((const uint16_t*)p.bias)[min(n + c, p.N - 1)];
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) raw[c] = ((const uint32_t*)p.bias)[min(n + c, p.N - 1)];
+  }
 }
+__device__ __forceinline__ float int8_bias(const Int8Epilogue& p, uint32_t raw) { return __uint_as_float(p.bias_dtype == JLLM_BF16 ? raw << 16 : raw); }
 
 // A sum with its scales and bias. Every kernel rounds here alike (no product joined with an addition), so that a row's outputs have the same
 // bits from all of them.

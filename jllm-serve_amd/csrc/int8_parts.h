@@ -63,6 +63,8 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
     if (V == 4) was = int8_load4(p, m, n);
     else was[0] = ((const float*)p.out)[(size_t)m * p.ldo + n];
   }
+  uint32_t bias[V];
+  int8_load_bias(p, n, bias);
   int sum[MATS][V] = {};
 #pragma unroll 4
   for (int z = 0; z < parts; ++z)
@@ -76,7 +78,7 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
   const float sa = p.scales.a[m];
 #pragma unroll
   for (int c = 0; c < V; ++c) {
-    const float z = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, n + c));
+    const float z = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, bias[c]));
     y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.scales.w2[n + c], 0.f), p.gate) : z;
   }
   if (!GATED && p.epilogue == 1) y += was;
