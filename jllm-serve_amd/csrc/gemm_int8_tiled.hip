@@ -7,9 +7,10 @@
 // a second set and asks for its share of the stage that takes the place of the one it multiplies. One barrier a stage.
 //
 // What binds is the pipe through which a compute unit fills its LDS, and where there are few stages the launch, the first bytes and the sum
-// of the parts. Two workgroups of 64 x 64 or 64 x 128 share a compute unit. us inside a graph: 128 x 6,144 x 4,096 12.3 (64 x 64), 487 22.2 (128 x
-// 128; in 64 x 64 26.1), 320 x 12,288 x 4,096 gated 55 (64 x 128; the large tiles 46), 80 x 12,288 x 4,096 gated 28.6 (128 x 128), 1,000 x 2,048 x 2,048
-// 11.3. Measured and not kept, since others were never far behind: 128 x 64, 128 x 128 by four waves in a ring of two, 128 x 256 and 256 x 128
+// of the parts. Two workgroups of 64 x 64 or 64 x 128 share a compute unit. us inside a graph: 128 x 6,144 x 4,096 11.9 (64 x 64), 487 23.0 (128 x
+// 128; in 64 x 64 27.6), 320 x 12,288 x 4,096 gated 55.6 (64 x 128; the large tiles 43.7), 128 x 12,288 x 4,096 gated 28.5 (128 x 128), 1,000 x 2,048 x
+// 2,048 10.8, 80 x 601 x 13,824 gated 13.4 (64 x 64 in six parts; with K whole 35.9). The scales requested at the start instead of in front of the
+// outputs: the same or up to 6 % slower. Measured and not kept, since others were never far behind: 128 x 64, 128 x 128 by four waves in a ring of two, 128 x 256 and 256 x 128
 // here (the large tiles' forms are 1 to 2 % faster).
 //
 // K may be cut over gridDim.z: the parts leave their whole-number sums, and a second kernel adds them and makes the outputs.

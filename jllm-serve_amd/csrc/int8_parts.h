@@ -12,7 +12,8 @@ struct Int8Args {
 
 // Which tile workgroup b of rows x cols takes: workgroups b, b + 8, b + 16 .. share a die, which gets a run of neighbouring tiles, in
 // bands of eight columns, row by row inside a band, so that its L2 passes on fewer operands. us, bands of 2 / 4 / 8 / 16: 4,608 x 17,408 x 5,120
-// gated in tiles of 256 x 256 639 / 632 / 624 / 629, 8,192 rows 1,115 / 1,094 / 1,085 / 1,104; at most sizes the same.
+// gated in tiles of 256 x 256 639 / 632 / 624 / 629, 8,192 rows 1,115 / 1,094 / 1,085 / 1,104 (all before the outputs took less); at most sizes the
+// same.
 #define I8_BAND 8
 __device__ __forceinline__ void int8_die_tile(int b, int rows, int cols, int& row, int& col) {
   const int tiles = rows * cols, each = tiles >> 3, more = tiles & 7, die = b & 7;
