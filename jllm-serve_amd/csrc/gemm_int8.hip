@@ -7,7 +7,7 @@
 // whole-number sums, and a second kernel adds them and makes the outputs.
 //
 // Bound by the loads' latency where there are few workgroups and by LDS where there are many: a stage takes 0.42 us for each workgroup that a
-// compute unit has. us inside a graph: 77 x 2,051 x 1,037 7.2 (with the scales and outputs one by one 9.7; besides, one stage ahead and
+// compute unit has. us inside a graph: 77 x 2,051 x 1,037 8.2 (with the scales and outputs one by one 9.7; besides, one stage ahead and
 // the last bytes by branches 14.7), 64 x 4,096 x 12,288 23
 // in four parts (the weight-streaming kernel 17), 2,048 x 4,096 x 4,096 114 (the large tiles 34: operands of many rows are laid out anew for them).
 #include <type_traits>
