@@ -1006,6 +1006,7 @@ def _int8_choices(units: int, N: int, K: int, gated: bool):
     return tuple((us, "jllm_gemm_int8_large" if tile >= INT8_LARGE_FROM else "jllm_gemm_int8_tiled", tile, parts) for us, tile, parts in found)
 
 
+@functools.lru_cache(maxsize=16384)
 def _int8_plans(M: int, N: int, K: int, gated: bool):
     """(estimated us, entry point, its tile or weight rows, parts of K) of the fast kernels for a product, the cheapest first."""
     if M <= INT8_STREAM_MOST_ROWS:
