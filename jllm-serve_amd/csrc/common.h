@@ -183,6 +183,9 @@ int jllm_splitk_reduce_norm(const float* partial, int splits, const void* bias, 
     if (e_ != hipSuccess) JLLM_FAIL("%s: launch failed: %s", name, hipGetErrorString(e_)); \
   } while (0)
 
+// Workgroups of `threads` that one launch may have: a grid of 2^32 threads or more is not refused, its size wraps, and what is left over does not run
+static inline unsigned jllm_most_groups(int threads) { return 0xffffffffu / (unsigned)threads; }
+
 #define JLLM_DISPATCH_1(code, T, ...)                 \
   if ((code) == JLLM_F32) {                           \
     typedef float T;                                  \

@@ -199,24 +199,40 @@ __global__ __launch_bounds__(THREADS) void int8_rows_kernel(RowsArgs p) {
   }
 }
 
+// A workgroup a row, in as many launches as the rows take
+template <bool NORM, bool ADD, typename TX, typename TA, typename TG, int J, int THREADS>
+int launch_rows_of(RowsArgs a, int rows, hipStream_t stream) {
+  const int most = (int)jllm_most_groups(THREADS);
+  for (; rows > 0; rows -= most) {
+    int8_rows_kernel<NORM, ADD, TX, TA, TG, J, THREADS><<<min(rows, most), THREADS, 0, stream>>>(a);
+    JLLM_CHECK_LAUNCH("int8_rows");
+    if (rows <= most) break;
+    const size_t n = (size_t)most;
+    a.x = (const TX*)a.x + n * a.ldx;
+    if (ADD) a.add = (const TA*)a.add + n * a.ld_add;
+    if (ADD) a.sum += n * a.ld_sum;
+    a.q += n * a.ldq;
+    a.scale += n;
+  }
+  return 0;
+}
+
 // Threads of a row and pieces of a thread by width
 template <bool NORM, bool ADD, typename TX, typename TA, typename TG>
 int launch_rows(const RowsArgs& a, int rows, hipStream_t stream) {
-#define I8_ROWS(J, THREADS) int8_rows_kernel<NORM, ADD, TX, TA, TG, J, THREADS><<<rows, THREADS, 0, stream>>>(a)
+#define I8_ROWS(J, THREADS) return launch_rows_of<NORM, ADD, TX, TA, TG, J, THREADS>(a, rows, stream)
   const int d = a.width;
   if (d < 8 || d > 32768) I8_ROWS(0, 256);
-  else if (d <= 512) I8_ROWS(1, 64);
-  else if (d <= 1024) I8_ROWS(2, 64);
-  else if (d <= 2048) I8_ROWS(1, 256);
-  else if (d <= 4096) I8_ROWS(2, 256);
-  else if (d <= 6144) I8_ROWS(3, 256);
-  else if (d <= 8192) I8_ROWS(4, 256);
-  else if (d <= 16384) I8_ROWS(2, 1024);
-  else if (d <= 24576) I8_ROWS(3, 1024);
-  else I8_ROWS(4, 1024);
+  if (d <= 512) I8_ROWS(1, 64);
+  if (d <= 1024) I8_ROWS(2, 64);
+  if (d <= 2048) I8_ROWS(1, 256);
+  if (d <= 4096) I8_ROWS(2, 256);
+  if (d <= 6144) I8_ROWS(3, 256);
+  if (d <= 8192) I8_ROWS(4, 256);
+  if (d <= 16384) I8_ROWS(2, 1024);
+  if (d <= 24576) I8_ROWS(3, 1024);
+  I8_ROWS(4, 1024);
 #undef I8_ROWS
-  JLLM_CHECK_LAUNCH("int8_rows");
-  return 0;
 }
 
 }  // namespace
@@ -264,14 +280,21 @@ extern "C" int jllm_dequantize_rows(const void* q, int ldq, const float* scale, 
   if (rows <= 0) return 0;
   if (width <= 0 || width > (1 << 30) || ldq < 0 || ldo < width) JLLM_FAIL("dequantize_rows: rows of %d, %d and %d apart", width, ldq, ldo);
   const int v = width < 8 ? 1 : 8, pieces = (width + v - 1) / v;
-  const size_t groups = ((size_t)rows * pieces + 255) / 256;
-  if (groups > 0x7fffffffull) JLLM_FAIL("dequantize_rows: %d rows of %d are more than a grid takes", rows, width);
+  const unsigned fit = jllm_most_groups(256) * 256u / (unsigned)pieces;
+  const int most = fit > 0x7fffffffu ? 0x7fffffff : (int)fit;  // rows that one launch has threads for
   JLLM_DISPATCH_1(out_dtype, TO, {
-    if (v == 8)
-      dequantize_rows_kernel<TO, 8><<<(unsigned)groups, 256, 0, stream>>>((const signed char*)q, ldq, scale, (TO*)out, ldo, rows, width, pieces);
-    else
-      dequantize_rows_kernel<TO, 1><<<(unsigned)groups, 256, 0, stream>>>((const signed char*)q, ldq, scale, (TO*)out, ldo, rows, width, pieces);
+    for (int first = 0; rows > 0; rows -= most, first += most) {
+      const int n = min(rows, most);
+      const unsigned groups = (unsigned)(((size_t)n * pieces + 255) / 256);
+      const signed char* from = (const signed char*)q + (size_t)first * ldq;
+      TO* to = (TO*)out + (size_t)first * ldo;
+      if (v == 8)
+        dequantize_rows_kernel<TO, 8><<<groups, 256, 0, stream>>>(from, ldq, scale + first, to, ldo, n, width, pieces);
+      else
+        dequantize_rows_kernel<TO, 1><<<groups, 256, 0, stream>>>(from, ldq, scale + first, to, ldo, n, width, pieces);
+      JLLM_CHECK_LAUNCH("dequantize_rows");
+      if (rows <= most) break;  // (first + most may not fit)
+    }
   })
-  JLLM_CHECK_LAUNCH("dequantize_rows");
   return 0;
 }
