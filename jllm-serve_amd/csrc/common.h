@@ -185,6 +185,9 @@ int jllm_splitk_reduce_norm(const float* partial, int splits, const void* bias, 
 
 // Workgroups of `threads` that one launch may have: a grid of 2^32 threads or more is not refused, its size wraps, and what is left over does not run
 static inline unsigned jllm_most_groups(int threads) { return 0xffffffffu / (unsigned)threads; }
+static inline bool jllm_grid_fits(dim3 grid, int threads) {
+  return grid.y <= 65535 && grid.z <= 65535 && (unsigned long long)grid.x * grid.y <= jllm_most_groups(threads) / grid.z;
+}
 
 #define JLLM_DISPATCH_1(code, T, ...)                 \
   if ((code) == JLLM_F32) {                           \

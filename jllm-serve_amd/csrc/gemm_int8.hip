@@ -139,8 +139,8 @@ extern "C" int jllm_gemm_int8(const void* A, int lda, const float* a_scale, cons
   const int each = (stages + parts - 1) / parts;
   parts = (stages + each - 1) / each;  // those that have any stage
   if (parts > 1 && (!partial || ((uintptr_t)partial & 15))) JLLM_FAIL("gemm_int8: %d parts of K need a buffer for their sums", parts);
-  const dim3 grid(W2 ? (N + 31) / 32 : (N + 63) / 64, (M + 63) / 64, parts);
-  if (grid.y > 65535) JLLM_FAIL("gemm_int8: %d rows are more than a grid takes", M);
+  const dim3 grid((N - 1) / (W2 ? 32 : 64) + 1, (M - 1) / 64 + 1, parts);
+  if (!jllm_grid_fits(grid, 256)) JLLM_FAIL("gemm_int8: %d x %d outputs are more than a grid takes", M, N);
   const Gemm8Args a{(const signed char*)A, (const signed char*)W, (const signed char*)W2, partial, lda, ldw, ldw2, K, each,
                     {{a_scale, w_scale, w2_scale}, bias, out, bias_dtype, out_dtype, ldo, M, N, epilogue, gs}};
   if (W2 && K < 16)
@@ -177,9 +177,14 @@ __global__ __launch_bounds__(256) void int8_lay_out_kernel(const signed char* __
 extern "C" int jllm_int8_lay_out(const void* src, int ld, void* dst, int ldd, int rows, int width, hipStream_t stream) {
   if (rows <= 0) return 0;
   if (width <= 0 || ld < 0 || ldd < width || (ldd & 15) || ((uintptr_t)dst & 15)) JLLM_FAIL("int8_lay_out: rows of %d, %d and %d apart", width, ld, ldd);
-  const size_t groups = ((size_t)rows * (ldd / 16) + 255) / 256;
-  if (groups > 0x7fffffffull) JLLM_FAIL("int8_lay_out: %d rows of %d are more than a grid takes", rows, width);
-  int8_lay_out_kernel<<<(unsigned)groups, 256, 0, stream>>>((const signed char*)src, ld, (signed char*)dst, ldd, rows, width);
-  JLLM_CHECK_LAUNCH("int8_lay_out");
+  const unsigned pieces = (unsigned)ldd / 16, fit = jllm_most_groups(256) * 256u / pieces;
+  const int most = fit > 0x7fffffffu ? 0x7fffffff : (int)fit;  // rows that one launch has threads for
+  for (int first = 0; rows > 0; rows -= most, first += most) {
+    const int n = min(rows, most);
+    int8_lay_out_kernel<<<(unsigned)(((size_t)n * pieces + 255) / 256), 256, 0, stream>>>((const signed char*)src + (size_t)first * ld, ld,
+                                                                                        (signed char*)dst + (size_t)first * ldd, ldd, n, width);
+    JLLM_CHECK_LAUNCH("int8_lay_out");
+    if (rows <= most) break;  // (first + most may not fit)
+  }
   return 0;
 }

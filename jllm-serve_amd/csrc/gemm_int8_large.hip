@@ -212,8 +212,8 @@ template <int FM, int WGM>
 static int launch_int8_large(const Int8Args& a, int parts, hipStream_t stream) {
   constexpr int TBM = WGM * FM * 32, TBN = L8_WAVES / WGM * 64;
   const int cols = a.W2 ? TBN / 2 : TBN;
-  const dim3 grid((a.end.N + cols - 1) / cols, (a.end.M + TBM - 1) / TBM, parts);
-  if (grid.y > 65535 || (unsigned long long)grid.x * grid.y > 0x7fffffffull) return 1;
+  const dim3 grid((a.end.N - 1) / cols + 1, (a.end.M - 1) / TBM + 1, parts);
+  if (!jllm_grid_fits(grid, L8_WAVES * 64)) return 1;
   constexpr size_t smem = Int8Ring<FM, WGM>::BYTES;
   if (!(a.W2 ? int8_allow_lds<gemm_int8_large_kernel<true, FM, WGM>>((int)smem) : int8_allow_lds<gemm_int8_large_kernel<false, FM, WGM>>((int)smem)))
     JLLM_FAIL("gemm_int8_large: cannot reserve %zu bytes of LDS", smem);

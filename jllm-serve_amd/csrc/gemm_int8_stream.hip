@@ -259,11 +259,11 @@ extern "C" int jllm_gemm_int8_stream(const void* A, int lda, const float* a_scal
   parts = parts < 1 ? 1 : parts > blocks ? blocks : parts;
   const int each = (blocks + parts - 1) / parts;
   parts = (blocks + each - 1) / each;  // those that have any block
-  if (parts > 65535) return 1;
+  const dim3 grid((N - 1) / rows + 1, parts);
+  if (!jllm_grid_fits(grid, 256)) return 1;
   if (parts > 1 && (!partial || ((uintptr_t)partial & 15))) JLLM_FAIL("gemm_int8_stream: %d parts of K need a buffer for their sums", parts);
   const Stream8Args a{(const signed char*)A, (const signed char*)W, (const signed char*)W2, partial, lda, ldw, K, rows, each,
                       {{a_scale, w_scale, w2_scale}, bias, out, bias_dtype, out_dtype, ldo, M, N, epilogue, gs}};
-  const dim3 grid((N + rows - 1) / rows, parts);
   const int rc = W2 ? launch_stream8_batch<true>(a, grid, stream) : launch_stream8_batch<false>(a, grid, stream);
   if (rc != 0) return rc;
   JLLM_CHECK_LAUNCH("gemm_int8_stream");

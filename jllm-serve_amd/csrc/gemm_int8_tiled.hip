@@ -169,8 +169,8 @@ template <bool GATED, int RM, int CN, int WGM, int WGN, int NS>
 static int launch_int8_tiled(const Int8Args& a, int parts, hipStream_t stream) {
   constexpr int TBM = WGM * RM * 16, TBN = WGN * CN * 16, COLS = GATED ? TBN / 2 : TBN, LDS = (TBM + TBN) * T8_ROW_BYTES * NS;
   static_assert(LDS <= 160 * 1024, "the ring fits");
-  const dim3 grid((a.end.N + COLS - 1) / COLS, (a.end.M + TBM - 1) / TBM, parts);
-  if (grid.y > 65535 || (unsigned long long)grid.x * grid.y > 0x7fffffffull) return 1;
+  const dim3 grid((a.end.N - 1) / COLS + 1, (a.end.M - 1) / TBM + 1, parts);
+  if (!jllm_grid_fits(grid, WGM * WGN * 64)) return 1;
   if (!int8_allow_lds<gemm_int8_tiled_kernel<GATED, RM, CN, WGM, WGN, NS>>(LDS))
     JLLM_FAIL("gemm_int8_tiled: cannot reserve %d bytes of LDS", LDS);
   // No more of the ring than the stages there are and the one behind them, whose bytes are read and not used: then more workgroups share a compute

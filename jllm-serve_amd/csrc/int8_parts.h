@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
 static inline int int8_add_parts(const int* partial, int parts, const Int8Epilogue& end, bool gated, hipStream_t stream) {
   const int v = end.N % 4 == 0 ? 4 : 1;
   const size_t groups = ((size_t)end.M * end.N / v + 255) / 256;
-  if (groups > 0x7fffffffull) JLLM_FAIL("gemm_int8: %d x %d outputs are more than a grid takes", end.M, end.N);
+  if (groups > jllm_most_groups(256)) JLLM_FAIL("gemm_int8: %d x %d outputs are more than a grid takes", end.M, end.N);
   const unsigned n = (unsigned)groups;
   if (gated) {
     if (v == 4) int8_parts_kernel<4, true><<<n, 256, 0, stream>>>(partial, parts, end);

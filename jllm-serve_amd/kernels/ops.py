@@ -707,6 +707,9 @@ class Int8Rows:
     def shape(self) -> torch.Size:
         return torch.Size(self._sizes[:2])
 
+    def _part(self, which: slice) -> "Int8Rows":
+        return Int8Rows(self.q[which], self.scale[which])
+
     def tensor(self, dtype: torch.dtype) -> torch.Tensor:
         """The values that the rows stand for, rounded once to ``dtype``."""
         code = _code(dtype)
@@ -720,6 +723,9 @@ class Int8Rows:
 
 
 INT8_MOST_INPUTS = 131071  # of a product: 128^2 times as many stay below 2^31, so every sum is exact
+# Of one launch, whatever kernel and tile it goes through: a grid has at most 65,535 tiles of 64 rows above each other and fewer than 2^32 threads,
+# 256 of them for eight weight rows (up to 64 rows), or for 64 x 64 sums
+INT8_MOST_ROWS, INT8_MOST_OUTPUTS, INT8_MOST_SUMS = 1 << 21, 1 << 26, 1 << 34
 
 
 # (These products take a few microseconds, and so does the host for each: what follows asks a tensor for its sizes once.)
@@ -874,6 +880,17 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
         out_code = _code(out.dtype)
         _here(*operands, bias, out)
     if M == 0 or N == 0:
+        return out
+    if M > INT8_MOST_ROWS or N > INT8_MOST_OUTPUTS or M * N > INT8_MOST_SUMS:
+        columns = min(N, INT8_MOST_OUTPUTS)
+        height = min(INT8_MOST_ROWS, INT8_MOST_SUMS // columns)
+        for n in range(0, N, columns):
+            c = slice(n, n + columns)
+            of = bias if bias is None else bias.view(-1)[c]
+            for m in range(0, M, height):
+                r = slice(m, m + height)
+                gemm_int8(a._part(r), w._part(c), w2=w2._part(c) if gated else None, bias=of, out=out[r, c], epilogue=int(epilogue) & 0xff, gate=gate,
+                          gate_limit=gate_limit)
         return out
     (rows, a_scale), (first, w_scale), (second, u_scale) = a._addresses(), w._addresses(), w2._addresses() if gated else (None, None)
     # what the fast kernels ask of the weights; whatever else does not fit them is laid out anew, or goes to the general kernel

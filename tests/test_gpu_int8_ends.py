@@ -1,4 +1,6 @@
 """The operators on rows of 8-bit integers at the ends of what they take."""
+import math
+
 import pytest
 import torch
 
@@ -71,3 +73,29 @@ def test_values_beyond_one_launch(ops):
     few = ops.quantize_rows(normal(seeded(7), 1000, width))
     got = ops.Int8Rows(repeated(few.q, rows), repeated(few.scale, rows)).tensor(torch.bfloat16)
     assert same(got, few.tensor(torch.bfloat16))
+
+
+@pytest.mark.parametrize("K", [64, 128, 50, 200])
+def test_products_of_more_rows_than_a_grid_has(ops, K):
+    """Tiles of 64 rows, of which a grid takes 65,535 above each other; K for the fast kernels and for the general one."""
+    gen = seeded(K)
+    M, N = 5_000_000, 16
+    a = ops.quantize_rows(normal(gen, 1000, K))
+    many = ops.Int8Rows(repeated(a.q, M), repeated(a.scale, M))
+    w, w2 = (ops.quantize_rows(normal(gen, N, K) / math.sqrt(K)) for _ in range(2))
+    bias, base = normal(gen, N), normal(gen, 1000, N)
+    assert same(ops.gemm_int8(many, w, bias=bias), ops.gemm_int8(a, w, bias=bias))
+    assert same(ops.gemm_int8(many, w, w2=w2, epilogue=ops.EPI_GATED), ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED))
+    out = repeated(base, M)
+    assert ops.gemm_int8(many, w, out=out, epilogue=ops.EPI_ADD) is out
+    assert same(out, ops.gemm_int8(a, w, out=base.clone(), epilogue=ops.EPI_ADD))
+
+
+@pytest.mark.parametrize("N,K", [((1 << 27) + 700, 16), ((1 << 30) + 64, 1)])
+def test_products_of_more_outputs_than_a_grid_has(ops, N, K):
+    gen = seeded(K)
+    w = ops.quantize_rows(normal(gen, 1000, K))
+    many = ops.Int8Rows(repeated(w.q, N), repeated(w.scale, N))
+    a, bias = ops.quantize_rows(normal(gen, 1, K)), normal(gen, 1000)
+    got = ops.gemm_int8(a, many, bias=repeated(bias, N))
+    assert same(got[0], ops.gemm_int8(a, w, bias=bias)[0])
