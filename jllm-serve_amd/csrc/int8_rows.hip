@@ -94,12 +94,23 @@ __device__ __forceinline__ uint32_t rounded(float y, const Rounding& r) {
   return r.inv == 0.f ? 0u : __float_as_uint(t + 12582912.0f) & 0xffu;
 }
 
-// The norm's scale. Squares and their sum are in 64 bits, where the squares are exact and none overflows: the kernel waits for memory
-// meanwhile, and a scale that is off by one unit turns whole numbers that lie near a half.
-__device__ __forceinline__ float rms_scale(double squares, int n, float eps) { return (float)(1.0 / sqrt(squares / n + (double)eps)); }
+// The norm's scale r, rounded once from 64 bits. Squares and their sum are in 64 bits, where the squares are exact and none overflows: the kernel waits
+// for memory meanwhile, and a scale that is off by one unit turns whole numbers that lie near a half. Rows whose root mean square lies beyond 2^100
+// or below 2^-100 are multiplied by a power of two first (exact, but for what is zero beside the row's largest): r itself may lie below
+// fp32's normal numbers there, or beyond them. A row of zeros without an eps has no root: its entries stay zeros.
+struct NormScale {
+  float pre, r;
+};
+__device__ __forceinline__ NormScale rms_scale(double squares, int n, float eps) {
+  const double mean = squares / n + (double)eps;
+  NormScale s;
+  s.pre = mean > 0x1p200 ? 0x1p-32f : mean < 0x1p-200 ? 0x1p64f : 1.0f;
+  s.r = mean == 0.0 ? 0.f : (float)(1.0 / sqrt(mean) / s.pre);
+  return s;
+}
 
 // Every entry of a norm is (h * r) * gain, two roundings
-__device__ __forceinline__ float normed(float h, float r, float g) { return (h * r) * g; }
+__device__ __forceinline__ float normed(float h, NormScale s, float g) { return ((h * s.pre) * s.r) * g; }
 
 template <bool NORM, bool ADD, typename TX, typename TA, typename TG, int J, int THREADS>
 __global__ __launch_bounds__(THREADS) void int8_rows_kernel(RowsArgs p) {
@@ -146,7 +157,7 @@ __global__ __launch_bounds__(THREADS) void int8_rows_kernel(RowsArgs p) {
         }
       }
       ss = row_sum<NW>(ss, red_sum);
-      const float r = rms_scale(ss, d, p.eps);
+      const NormScale r = rms_scale(ss, d, p.eps);
       if (ADD) {  // behind the barrier: every thread has its overlapping entries of the old row
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -177,7 +188,7 @@ __global__ __launch_bounds__(THREADS) void int8_rows_kernel(RowsArgs p) {
     return;
   } else {
     // A row of any width, entry by entry; a thread reads again what it alone wrote
-    float r = 0.f;
+    NormScale r{};
     if (NORM) {
       double ss = 0.0;
       for (int i = tid; i < d; i += THREADS) {

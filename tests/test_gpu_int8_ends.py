@@ -4,9 +4,12 @@ import math
 import pytest
 import torch
 
+import int8_oracle as oracle
+
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
+NORM_SCALE, NORM_ENTRY = 5, 6  # fp32 roundings of a norm's scale and of an entry against its row's largest
 
 
 @pytest.fixture(scope="module")
@@ -99,3 +102,25 @@ def test_products_of_more_outputs_than_a_grid_has(ops, N, K):
     a, bias = ops.quantize_rows(normal(gen, 1, K)), normal(gen, 1000)
     got = ops.gemm_int8(a, many, bias=repeated(bias, N))
     assert same(got[0], ops.gemm_int8(a, w, bias=bias)[0])
+
+
+# ------------------------------------------------------------------------------------------------ values at the ends of fp32
+
+
+@pytest.mark.parametrize("width", [5, 40, 1031, 5120, 33000])
+@pytest.mark.parametrize("added", [False, True])
+def test_norm_at_the_ends_of_fp32(ops, width, added):
+    """Rows near fp32's largest, whose inverse root mean square lies below its normal numbers; with an eps of zero rows below them, whose
+    inverse is beyond its largest, and rows of zeros."""
+    gen = seeded(width)
+    tens = torch.tensor([3e38, 1e38, 1e30, 1.0, 1e-30, 1e-38, 1e-42, 0.0], dtype=torch.float64)
+    x = (torch.rand(8, width, generator=gen, device=DEV).double().cpu() * 1.8 - 0.9).clamp(-0.9, 0.9)
+    x[:, width // 2] = 0.95
+    x = (x * tens[:, None]).float().to(DEV)
+    gain = 1 + 0.1 * normal(gen, width)
+    add = x * 0.0625 if added else None
+    h, _ = oracle.norm(x[:7], gain, 0.0, None if add is None else add[:7])
+    y = oracle.norm(h, gain, 0.0)[1]
+    got = ops.rmsnorm_int8(x, gain, 0.0, add=add, out=torch.empty_like(x) if added else None)
+    oracle.check_rows(got.q[:7], got.scale[:7], y, NORM_ENTRY, NORM_SCALE)
+    assert float(got.scale[7]) == 0 and not got.q[7].any()
