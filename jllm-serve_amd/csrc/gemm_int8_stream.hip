@@ -197,11 +197,12 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
       for (int u = 0; u < MATS; ++u)
         int8_part_store(p.partial + ((size_t)blockIdx.y * MATS + u) * M * N, it.m, it.n, it.there, N, sum[u]);
     } else {
+      const Int8RowScale sa = int8_row_scale(it.sa);
       floatx4 y;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float z = int8_output(sum[0][c], it.sa, it.sw[c], int8_bias(p.end, it.bias[c]));
-        y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], it.sa, it.su[c], 0.f), p.end.gate) : z;
+        const float z = int8_output(sum[0][c], sa, it.sw[c], int8_bias(p.end, it.bias[c]));
+        y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, it.su[c], 0.f), p.end.gate) : z;
       }
       if (!GATED && p.end.epilogue == 1) y += it.was;
       int8_store4(p.end, it.m, it.n, it.there, y);

@@ -5,8 +5,8 @@
 // half the depth (mfma.h), and it takes as many clocks.
 //
 // The sums are exact (up to 131,071 inputs, where 128^2 K stays below 2^31), so an output does not depend on the tile, the cut of
-// K or the order in which parts are added. It is (float(sum) * a_scale[m]) * w_scale[n], and from there on what the other
-// products make of a sum.
+// K or the order in which parts are added. It is (float(sum) * a_scale[m]) * w_scale[n] without an overflow in between, and from there
+// on what the other products make of a sum.
 #pragma once
 #include <atomic>
 #include "common.h"
@@ -52,11 +52,19 @@ __device__ __forceinline__ void int8_load_bias(const Int8Epilogue& p, int n, uin
 }
 __device__ __forceinline__ float int8_bias(const Int8Epilogue& p, uint32_t raw) { return __uint_as_float(p.bias_dtype == JLLM_BF16 ? raw << 16 : raw); }
 
+// A row's scale as its sums are multiplied by it: from 2^96 on a sum's product with it may be beyond fp32 where the channel's scale brings the output
+// back, so 2^32 of it waits until then (exact on both ways: sums are whole numbers, so nothing falls below fp32's normal numbers meanwhile)
+#define I8_FAR 0x1p96f
+struct Int8RowScale {
+  float a, back;
+};
+__device__ __forceinline__ Int8RowScale int8_row_scale(float sa) { return sa >= I8_FAR ? Int8RowScale{sa * 0x1p-32f, 0x1p32f} : Int8RowScale{sa, 1.0f}; }
+
 // A sum with its scales and bias. Every kernel rounds here alike (no product joined with an addition), so that a row's outputs have the same
 // bits from all of them.
-__device__ __forceinline__ float int8_output(int sum, float sa, float sw, float b) {
+__device__ __forceinline__ float int8_output(int sum, Int8RowScale s, float sw, float b) {
 #pragma clang fp contract(off)
-  const float y = ((float)sum * sa) * sw;
+  const float y = (((float)sum * s.a) * sw) * s.back;
   return y + b;
 }
 
@@ -108,7 +116,7 @@ __device__ __forceinline__ void int8_columns(const float* from, int n, int N, bo
 
 // A wave's accumulators, CN runs of four columns for each of its RM blocks of 16 rows (gated: [.][j] and [.][j + CN / 2] are the two weights' of the
 // same outputs), row block by row block, so that hardly more than the sums themselves is in registers. Where all of its columns are there
-// it goes without a branch per output, and everything is requested before the first output is stored (behind a store the compiler moves no
+// (and no row's scale is far beyond others') it goes without a branch per output, and everything is requested before the first output is stored (behind a store the compiler moves no
 // load forward, and each would wait for its own way); what the outputs are added to, one block of rows ahead.
 template <bool GATED, int FN, int RM, int CN>
 __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
@@ -137,16 +145,20 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
 #pragma unroll
     for (int j = 0; j < NI; ++j) int8_columns((const float*)p.bias, col0 + j * 16, p.N, whole, bv[j]);
   }
-  auto outputs = [&](int i, int j) {
+  auto scaled = [&](int i, int j, Int8RowScale s) {
     floatx4 v;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const float z = int8_output(acc[i][j][c], sa[i], sw[j][c], bv[j][c]);
-      v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], sa[i], su[j][c], 0.f), GateSpec{FN, p.gate.limit}) : z;
+      const float z = int8_output(acc[i][j][c], s, sw[j][c], bv[j][c]);
+      v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], s, su[j][c], 0.f), GateSpec{FN, p.gate.limit}) : z;
     }
     return v;
   };
-  if (!whole) {
+  auto outputs = [&](int i, int j) { return scaled(i, j, Int8RowScale{sa[i], 1.0f}); };
+  float most = sa[0];  // of a row's scale in this wave
+#pragma unroll
+  for (int i = 1; i < RM; ++i) most = fmaxf(most, sa[i]);
+  if (!whole || __any(most >= I8_FAR)) {
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
       const int m = row0 + i * 16;
@@ -155,7 +167,7 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
       for (int j = 0; j < NI; ++j) {
         const int n = col0 + j * 16;
         if (n >= p.N) continue;
-        floatx4 v = outputs(i, j);
+        floatx4 v = scaled(i, j, int8_row_scale(sa[i]));
         if (!GATED && p.epilogue == 1) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) v[c] += ((const float*)p.out)[(size_t)m * p.ldo + min(n + c, p.N - 1)];

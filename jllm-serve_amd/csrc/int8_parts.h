@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
 #pragma unroll
       for (int c = 0; c < V; ++c) sum[u][c] += s[c];
     }
-  const float sa = p.scales.a[m];
+  const Int8RowScale sa = int8_row_scale(p.scales.a[m]);
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     const float z = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, bias[c]));

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import int8_oracle as oracle
+from int8_oracle import U
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +125,42 @@ def test_norm_at_the_ends_of_fp32(ops, width, added):
     got = ops.rmsnorm_int8(x, gain, 0.0, add=add, out=torch.empty_like(x) if added else None)
     oracle.check_rows(got.q[:7], got.scale[:7], y, NORM_ENTRY, NORM_SCALE)
     assert float(got.scale[7]) == 0 and not got.q[7].any()
+
+
+KERNELS = [("", 0, 1)] + [(kernel, size, parts) for kernel, size in (("jllm_gemm_int8_stream", 24), ("jllm_gemm_int8_tiled", 64064), ("jllm_gemm_int8_tiled", 128128),
+                                                                     ("jllm_gemm_int8_large", 256256)) for parts in (1, 3)]
+
+
+@pytest.mark.parametrize("kernel,size,parts", KERNELS)
+@pytest.mark.parametrize("N", [256, 203])
+def test_products_of_rows_near_the_largest(ops, monkeypatch, kernel, size, parts, N):
+    """Rows whose scale times the sum is beyond fp32, which the channel's scale brings back; the rows beside them keep their bits."""
+    gen = seeded(N)
+    M, K = 64 if kernel.endswith("stream") else 150, 1040
+    x = normal(gen, M, K).clamp(-4, 4)
+    far = torch.arange(M, device=DEV) % 3 == 1
+    x[far] *= torch.tensor([8e37, 1e35, 1e30], device=DEV).repeat(M)[:int(far.sum()), None]
+    a = ops.quantize_rows(x)
+    w = ops.quantize_rows(normal(gen, N, K) * 1e-12)
+    tiny, fine = ops.quantize_rows(normal(gen, N, K) * 1e-40), ops.quantize_rows(normal(gen, N, K))
+    bias, base = normal(gen, N), normal(gen, M, N)
+    monkeypatch.setattr(ops, "_int8_plans", lambda *args: ((0.0, kernel, size, parts),) if kernel else ())
+    for weight in (w, tiny):
+        y, tol = oracle.product(a, weight, bias)
+        got = ops.gemm_int8(a, weight, bias=bias, out_dtype=torch.float32).double().cpu()
+        assert torch.isfinite(got).all() and ((got - y).abs() <= tol).all()
+        y, tol = oracle.product(a, weight, None, base)
+        got = ops.gemm_int8(a, weight, out=base.clone(), epilogue=ops.EPI_ADD).double().cpu()
+        assert torch.isfinite(got).all() and ((got - y).abs() <= tol).all()
+    # gated: the row that is brought back into range, times a value that keeps it there (|z| to 1e30: the gate is 0 or z)
+    z, u = oracle.sums(a, w), oracle.sums(a, tiny)
+    y = oracle.gate("silu", z, u)
+    some = (z.abs() > 1e3) & (y.abs() < 1e38)
+    assert int(some.sum()) > N
+    got = ops.gemm_int8(a, w, w2=tiny, epilogue=ops.EPI_GATED, out_dtype=torch.float32).double().cpu()
+    assert ((got - y).abs() <= y.abs() * 16 * U + 1e-30)[some].all()
+    # and the others
+    near = ~far
+    alone = ops.Int8Rows(a.q[near], a.scale[near])
+    whole = ops.gemm_int8(a, fine, bias=bias)
+    assert torch.equal(whole[near], ops.gemm_int8(alone, fine, bias=bias))
