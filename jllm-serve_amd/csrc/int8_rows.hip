@@ -103,10 +103,9 @@ struct NormScale {
 };
 __device__ __forceinline__ NormScale rms_scale(double squares, int n, float eps) {
   const double mean = squares / n + (double)eps;
-  NormScale s;
-  s.pre = mean > 0x1p200 ? 0x1p-32f : mean < 0x1p-200 ? 0x1p64f : 1.0f;
-  s.r = mean == 0.0 ? 0.f : (float)(1.0 / sqrt(mean) / s.pre);
-  return s;
+  const bool large = mean > 0x1p200, small = mean < 0x1p-200;
+  const float r = (float)((large ? 0x1p32 : small ? 0x1p-64 : 1.0) / sqrt(mean));
+  return {large ? 0x1p-32f : small ? 0x1p64f : 1.0f, mean == 0.0 ? 0.f : r};
 }
 
 // Every entry of a norm is (h * r) * gain, two roundings
