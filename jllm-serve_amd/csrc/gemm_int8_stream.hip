@@ -200,9 +200,12 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_int8_stream_kernel(Stream8Arg
       const Int8RowScale sa = int8_row_scale(it.sa);
       floatx4 y;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float z = int8_output(sum[0][c], sa, it.sw[c], int8_bias(p.end, it.bias[c]));
-        y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, it.su[c], 0.f), p.end.gate) : z;
+      for (int c = 0; c < 4; ++c) y[c] = int8_output(sum[0][c], sa, it.sw[c], int8_bias(p.end, it.bias[c]));
+      if (GATED) {
+        floatx4 u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) u[c] = int8_output(sum[MATS - 1][c], sa, it.su[c], 0.f);
+        y = int8_gated4(y, u, p.end.gate, p.end.out_dtype);
       }
       if (!GATED && p.end.epilogue == 1) y += it.was;
       int8_store4(p.end, it.m, it.n, it.there, y);

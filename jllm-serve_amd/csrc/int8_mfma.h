@@ -68,10 +68,47 @@ __device__ __forceinline__ float int8_output(int sum, Int8RowScale s, float sw, 
   return y + b;
 }
 
-// The gate of two of them. Rows without numbers have a scale of NaN, and clamps would lose it.
+// 1 / (1 + exp(-slope x)), SLOPE in millionths, for outputs in fp32: the hardware's exp2 of the rounded exponent, times what the rounding left of it (by itself
+// that is |slope x| halves of a step), so that the exponential and the reciprocal are off by one unit each. The bounds of x change no result (2^x is 0
+// or infinite long before) and keep what is left a number.
+template <int SLOPE>
+__device__ __forceinline__ float int8_sigmoid(float x) {
+#pragma clang fp contract(off)
+  constexpr double RATE = SLOPE * 1e-6 * 1.4426950408889634074;
+  constexpr float HI = (float)RATE, LO = (float)(RATE - (double)HI);
+  x = fminf(fmaxf(x, -256.0f), 256.0f);
+  const float t = x * HI, left = fmaf(x, LO, fmaf(x, HI, -t));
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-t) * fmaf(left, -0.6931471805599453f, 1.0f));
+}
+
+// The gate of two of them; FINE: of an output in fp32, where common.h's fast form would show. Rows without numbers have a scale of NaN, and clamps
+// would lose it.
+template <bool FINE>
 __device__ __forceinline__ float int8_gated(float z, float u, GateSpec gs) {
-  const float y = gated<true>(z, u, gs);
+#pragma clang fp contract(off)
+  float y;
+  if (!FINE) {
+    y = gated<true>(z, u, gs);
+  } else if (gs.fn == JLLM_GATE_SILU) {
+    y = z * int8_sigmoid<1000000>(z) * u;
+  } else if (gs.fn == JLLM_GATE_GELU_TANH) {  // 0.5 (1 + tanh x) = 1 / (1 + exp(-2x))
+    y = z * int8_sigmoid<2000000>(0.7978845608028654f * (z + 0.044715f * z * z * z)) * u;
+  } else {
+    const float g = fminf(z, gs.limit), v = fminf(fmaxf(u, -gs.limit), gs.limit);
+    y = g * int8_sigmoid<1702000>(g) * (v + 1.0f);
+  }
   return gs.fn != JLLM_GATE_SWISH_CLAMPED || (z == z && u == u) ? y : z + u;
+}
+__device__ __forceinline__ floatx4 int8_gated4(floatx4 z, floatx4 u, GateSpec gs, int out_dtype) {
+  floatx4 y;
+  if (out_dtype == JLLM_BF16) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y[c] = int8_gated<false>(z[c], u[c], gs);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) y[c] = int8_gated<true>(z[c], u[c], gs);
+  }
+  return y;
 }
 
 // What four neighbouring outputs of row m from column n on are added to
@@ -118,7 +155,7 @@ __device__ __forceinline__ void int8_columns(const float* from, int n, int N, bo
 // same outputs), row block by row block, so that hardly more than the sums themselves is in registers. Where all of its columns are there
 // (and no row's scale is far beyond others') it goes without a branch per output, and everything is requested before the first output is stored (behind a store the compiler moves no
 // load forward, and each would wait for its own way); what the outputs are added to, one block of rows ahead.
-template <bool GATED, int FN, int RM, int CN>
+template <bool GATED, int FN, bool FINE, int RM, int CN>
 __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
   constexpr int NI = GATED ? CN / 2 : CN;
   const int group = lane / 16, row0 = m0 + wm * RM * 16 + lane % 16, col0 = n0 + wn * NI * 16 + group * 4;
@@ -150,7 +187,7 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const float z = int8_output(acc[i][j][c], s, sw[j][c], bv[j][c]);
-      v[c] = GATED ? int8_gated(z, int8_output(acc[i][GATED ? NI + j : 0][c], s, su[j][c], 0.f), GateSpec{FN, p.gate.limit}) : z;
+      v[c] = GATED ? int8_gated<FINE>(z, int8_output(acc[i][GATED ? NI + j : 0][c], s, su[j][c], 0.f), GateSpec{FN, p.gate.limit}) : z;
     }
     return v;
   };
@@ -193,7 +230,7 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
         __builtin_memcpy(out + (size_t)(row0 + i * 16) * p.ldo + j * 16, &v, 16);
       }
     }
-  } else if (p.out_dtype == JLLM_BF16) {
+  } else if (GATED ? !FINE : p.out_dtype == JLLM_BF16) {
     bf16_t* out = (bf16_t*)p.out + col0;
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
@@ -232,15 +269,22 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
   }
 }
 
-// The same, each gate function in code of its own: chosen output by output it took as long as the gates themselves
+// The same, each gate function in code of its own for outputs in bf16 and in fp32: chosen output by output it took as long as the gates themselves
 template <bool GATED, int RM, int CN>
 __device__ __forceinline__ void int8_epilogue(const intx4 (&acc)[RM][CN], int lane, int wm, int wn, int m0, int n0, const Int8Epilogue& p) {
-  if (!GATED || p.gate.fn == JLLM_GATE_SILU)
-    int8_outputs<GATED, JLLM_GATE_SILU>(acc, lane, wm, wn, m0, n0, p);
-  else if (p.gate.fn == JLLM_GATE_GELU_TANH)
-    int8_outputs<GATED, JLLM_GATE_GELU_TANH>(acc, lane, wm, wn, m0, n0, p);
-  else
-    int8_outputs<GATED, JLLM_GATE_SWISH_CLAMPED>(acc, lane, wm, wn, m0, n0, p);
+#define I8_OUTPUTS(FN)                                                           \
+  if (!GATED || p.out_dtype == JLLM_BF16)                                        \
+    int8_outputs<GATED, FN, false>(acc, lane, wm, wn, m0, n0, p);                \
+  else                                                                           \
+    int8_outputs<GATED, FN, true>(acc, lane, wm, wn, m0, n0, p)
+  if (!GATED || p.gate.fn == JLLM_GATE_SILU) {
+    I8_OUTPUTS(JLLM_GATE_SILU);
+  } else if (p.gate.fn == JLLM_GATE_GELU_TANH) {
+    I8_OUTPUTS(JLLM_GATE_GELU_TANH);
+  } else {
+    I8_OUTPUTS(JLLM_GATE_SWISH_CLAMPED);
+  }
+#undef I8_OUTPUTS
 }
 
 // Above 64 KB a kernel's dynamic LDS has to be allowed first, on every device once

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
   const size_t all = (size_t)p.M * p.N, i = ((size_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (i >= all) return;
   const int m = (int)(i / p.N), n = (int)(i - (size_t)m * p.N);
-  floatx4 y{0.f, 0.f, 0.f, 0.f}, was{0.f, 0.f, 0.f, 0.f};
+  floatx4 y{0.f, 0.f, 0.f, 0.f}, u = y, was = y;
   if (!GATED && p.epilogue == 1) {  // on its way together with the sums
     if (V == 4) was = int8_load4(p, m, n);
     else was[0] = ((const float*)p.out)[(size_t)m * p.ldo + n];
@@ -70,18 +70,19 @@ __global__ __launch_bounds__(256) void int8_parts_kernel(const int* __restrict__
 #pragma unroll 4
   for (int z = 0; z < parts; ++z)
 #pragma unroll
-    for (int u = 0; u < MATS; ++u) {
+    for (int w = 0; w < MATS; ++w) {
       int s[V];
-      __builtin_memcpy(s, (const int*)__builtin_assume_aligned(partial + ((size_t)z * MATS + u) * all + i, 4 * V), sizeof(s));
+      __builtin_memcpy(s, (const int*)__builtin_assume_aligned(partial + ((size_t)z * MATS + w) * all + i, 4 * V), sizeof(s));
 #pragma unroll
-      for (int c = 0; c < V; ++c) sum[u][c] += s[c];
+      for (int c = 0; c < V; ++c) sum[w][c] += s[c];
     }
   const Int8RowScale sa = int8_row_scale(p.scales.a[m]);
 #pragma unroll
   for (int c = 0; c < V; ++c) {
-    const float z = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, bias[c]));
-    y[c] = GATED ? int8_gated(z, int8_output(sum[MATS - 1][c], sa, p.scales.w2[n + c], 0.f), p.gate) : z;
+    y[c] = int8_output(sum[0][c], sa, p.scales.w[n + c], int8_bias(p, bias[c]));
+    if (GATED) u[c] = int8_output(sum[MATS - 1][c], sa, p.scales.w2[n + c], 0.f);
   }
+  if (GATED) y = int8_gated4(y, u, p.gate, p.out_dtype);
   if (!GATED && p.epilogue == 1) y += was;
   int8_store4(p, m, n, V, y);
 }

@@ -164,3 +164,37 @@ def test_products_of_rows_near_the_largest(ops, monkeypatch, kernel, size, parts
     alone = ops.Int8Rows(a.q[near], a.scale[near])
     whole = ops.gemm_int8(a, fine, bias=bias)
     assert torch.equal(whole[near], ops.gemm_int8(alone, fine, bias=bias))
+
+
+# ------------------------------------------------------------------------------------------------ gates in fp32
+
+
+@pytest.mark.parametrize("gate,limit", [("silu", 0.0), ("swish_clamped", 60.0), ("gelu_tanh", 0.0)])
+@pytest.mark.parametrize("M,N,K", [(3, 50, 70), (40, 256, 512), (64, 203, 640), (100, 256, 512), (130, 272, 2064), (300, 272, 528)])
+def test_gates_in_fp32(ops, gate, limit, M, N, K):
+    """A gated output in fp32 is as good as its two sums in fp32 allow: against the gate in 64 bits of those sums as they are rounded, whatever
+    their size.
+
+    2^x one unit (two halves), what its argument's rounding left one product with one rounding of its factor (3), 1 + that (1), the
+    reciprocal one unit (2), two products (2), (u + 1) (1): 11 halves of a step, where an argument rounded by itself costs |z| of them. gelu's argument
+    has 7 roundings of its own, times 2 |inner|. The reciprocal of more than 2^126 may be zero: what is lost lies below 128 * 2^-126 times |u|."""
+    gen = seeded(M + N)
+    a = ops.quantize_rows(normal(gen, M, K))
+    w, w2 = (ops.quantize_rows(normal(gen, N, K) * (25 if gate != "gelu_tanh" else 3) / math.sqrt(K)) for _ in range(2))
+
+    def sums(weight):  # as the kernels round them
+        s = (a.q.cpu().double() @ weight.q.cpu().double().t()).float()
+        return ((s * a.scale.cpu()[:, None]) * weight.scale.cpu()[None, :]).double()
+
+    z, u = sums(w), sums(w2)
+    assert float(z.abs().max()) > (60 if gate != "gelu_tanh" else 5)
+    y = oracle.gate(gate, z, u, limit)
+    tol = 11 * U * y.abs()
+    if gate == "gelu_tanh":  # 0.5 (1 + tanh x) as the sigmoid of 2x: where it is small, the sum has no digits left in 64 bits either
+        inner = 0.7978845608028654 * (z + 0.044715 * z ** 3)
+        y = z * torch.sigmoid(2 * inner) * u
+        tol = (11 + 14 * inner.abs()) * U * y.abs()
+    tol = tol * 1.01 + 128 * 2.0 ** -126 * (u.abs() + 1)
+    got = ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED, gate=ops.GATE_FUNCTIONS[gate], gate_limit=limit, out_dtype=torch.float32).double().cpu()
+    off = (got - y).abs() - tol
+    assert (off <= 0).all(), (float((got - y).abs().div(y.abs().clamp_min(1e-30)).max() / U), int((off > 0).sum()))
