@@ -306,6 +306,13 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _held(*tensors) -> None:
+    """What `_ptr` does beside giving the address, for functions that ask a tensor for it themselves."""
+    mine = getattr(_kept, "now", None)
+    if mine is not None:
+        mine.tensors += [t for t in tensors if t is not None]
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -717,6 +724,8 @@ class Int8Rows:
         _here(*self._tensors)
         out = _new_rows(n, width, dtype, self._tensors[0])
         if n and width:
+            if _keeping:
+                _held(*self._tensors, out)
             q, scale = self._addresses()
             _call("jllm_dequantize_rows", q, distance, scale, n, width, out.data_ptr(), code, out.stride(0), _stream())
         return out
@@ -792,6 +801,8 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     _here(x)
     rows = Int8Rows._new(n, width, x)
     if n:
+        if _keeping:
+            _held(x, *rows._tensors)
         q, scale = rows._addresses()
         _call("jllm_quantize_rows", x.data_ptr(), code, distance, n, width, q, width, scale, _stream())
     return rows
@@ -828,6 +839,8 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
         _here(x, gain, add, out)
     rows = Int8Rows._new(n, width, x)
     if n:
+        if _keeping:
+            _held(x, gain, add, out, *rows._tensors)
         q, scale = rows._addresses()
         _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, q, width, scale, _stream())
     return rows
@@ -892,6 +905,8 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
                 gemm_int8(a._part(r), w._part(c), w2=w2._part(c) if gated else None, bias=of, out=out[r, c], epilogue=int(epilogue) & 0xff, gate=gate,
                           gate_limit=gate_limit)
         return out
+    if _keeping:
+        _held(*operands, bias, out)
     (rows, a_scale), (first, w_scale), (second, u_scale) = a._addresses(), w._addresses(), w2._addresses() if gated else (None, None)
     # what the fast kernels ask of the weights; whatever else does not fit them is laid out anew, or goes to the general kernel
     if not (K | ldw | first) % 16 and (not gated or (ldu == ldw and not second % 16)):
@@ -923,13 +938,18 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
 
 def _int8_sums(M: int, N: int, gated: bool, parts: int, out: torch.Tensor) -> torch.Tensor:
     """Where the parts of a cut K leave their sums, of this product alone."""
-    return torch.empty((parts * M * N * (2 if gated else 1),), dtype=torch.int32, device=out.device)
+    sums = torch.empty((parts * M * N * (2 if gated else 1),), dtype=torch.int32, device=out.device)
+    if _keeping:
+        _held(sums)
+    return sums
 
 
 def _int8_laid_out(address: int, n: int, width: int, distance: int, beside: torch.Tensor):
     """(tensor, its address, entries between rows): the rows at ``address`` as the fast kernels take them, with zeros up to a multiple of 16."""
     padded = -(-width // 16) * 16
     new = torch.empty((n, padded), dtype=torch.int8, device=beside.device)
+    if _keeping:
+        _held(new)
     _call("jllm_int8_lay_out", address, distance, new.data_ptr(), padded, n, width, _stream())
     return new, new.data_ptr(), padded
 

@@ -67,3 +67,29 @@ def test_a_product_of_any_size_is_made_of_pieces_that_fit(monkeypatch, M, N, K, 
         pieces = sorted((r, m) for r, at, m, _ in done if at == c)
         assert [r for r, _ in pieces] == [sum(m for _, m in pieces[:i]) for i in range(len(pieces))] and sum(m for _, m in pieces) == M
     assert len(done) == 1 or M > ops.INT8_MOST_ROWS or N > ops.INT8_MOST_OUTPUTS or M * N > ops.INT8_MOST_SUMS
+
+
+@pytest.mark.parametrize("M,N,K,at", [(1, 64, 128, 0), (40, 96, 8192, 0), (40, 96, 8191, 0), (70, 64, 8192, 0), (70, 64, 128, 3), (600, 640, 2061, 0)])
+def test_kept_launches_keep_their_operands(monkeypatch, M, N, K, at):
+    """Every address that a kept launch was given lies in a tensor that is kept with it: operands, results, sums of a cut K, rows laid out anew."""
+    recorded.record(monkeypatch)
+    calls = []
+    monkeypatch.setattr(ops, "_try", lambda name, *args: calls.append((name, args)) or True)
+    monkeypatch.setattr(ops, "_call", lambda name, *args: calls.append((name, args)))
+    monkeypatch.setattr(ops, "_here", lambda *tensors: None)
+    with ops.kept_launches() as kept:
+        x = torch.empty(M * K + at, dtype=torch.float32)[at:].view(M, K)
+        a = ops.rmsnorm_int8(x, torch.empty(K), 1e-6, add=torch.empty((M, K)), out=torch.empty((M, K)))
+        ops.rmsnorm_int8(x, torch.empty(K), 1e-6)
+        w, w2 = (ops.Int8Rows(torch.empty(N * K + at, dtype=torch.int8)[at:].view(N, K), torch.empty(N)) for _ in range(2))
+        ops.gemm_int8(a, w, bias=torch.empty(N))
+        ops.gemm_int8(a, w, out=torch.empty((M, N)), epilogue=ops.EPI_ADD)
+        ops.quantize_rows(ops.gemm_int8(a, w, w2=w2, epilogue=ops.EPI_GATED)).tensor(torch.float32)
+    memory = [(t.untyped_storage().data_ptr(), t.untyped_storage().nbytes()) for t in kept.tensors]
+    assert len(calls) >= 7
+    for name, args in calls:
+        types = ops._SIGS.get(name) or ops._OPTIONAL_SIGS[name]
+        assert len(types) == len(args)
+        for i, (kind, value) in enumerate(zip(types[:-1], args)):  # (the last is the stream)
+            if kind is ops._P and value:
+                assert any(start <= value < start + size for start, size in memory), (name, i)
