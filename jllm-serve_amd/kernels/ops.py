@@ -842,7 +842,7 @@ def rmsnorm_int8(x: torch.Tensor, gain: torch.Tensor, eps: float, *, add: Option
         if _keeping:
             _held(x, gain, add, out, *rows._tensors)
         q, scale = rows._addresses()
-        _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, float(eps), q, width, scale, _stream())
+        _call("jllm_rmsnorm_int8", x.data_ptr(), distance, *joins, n, width, gain.data_ptr(), gain_code, eps, q, width, scale, _stream())
     return rows
 
 
@@ -924,7 +924,7 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
     else:
         plans = ()
     head = (rows, lda, a_scale, first, ldw, w_scale, second, ldu, u_scale,
-            bias.data_ptr() if bias is not None else None, bias_code, out.data_ptr(), out_code, ldo, M, N, K, int(epilogue), float(gate_limit))
+            bias.data_ptr() if bias is not None else None, bias_code, out.data_ptr(), out_code, ldo, M, N, K, epilogue, gate_limit)
     for _, kernel, size, parts in plans:
         sums = _int8_sums(M, N, gated, parts, out) if parts > 1 else None
         if _try(kernel, *head, size, parts, None if sums is None else sums.data_ptr(), _stream()):

@@ -93,22 +93,3 @@ def test_kept_launches_keep_their_operands(monkeypatch, M, N, K, at):
         for i, (kind, value) in enumerate(zip(types[:-1], args)):  # (the last is the stream)
             if kind is ops._P and value:
                 assert any(start <= value < start + size for start, size in memory), (name, i)
-
-
-def test_numbers_of_any_kind(monkeypatch):
-    """An eps, a limit and an epilogue may be numbers of another library, as for `rmsnorm` and `gemm`."""
-    import ctypes
-
-    import numpy
-    seen = recorded.record(monkeypatch)
-    monkeypatch.setattr(ops, "_here", lambda *tensors: None)
-    rows = lambda n: ops.Int8Rows(torch.empty((n, 64), dtype=torch.int8), torch.empty(n))
-    for number in (numpy.float32, numpy.float16, torch.tensor):
-        ops.rmsnorm_int8(torch.empty((3, 64)), torch.empty(64), number(0.5))
-        ops.gemm_int8(rows(3), rows(16), w2=rows(16), epilogue=numpy.int64(ops.EPI_GATED), gate=numpy.int64(2), gate_limit=number(0.5))
-        ops.gemm_int8(rows(3), rows(16), out=torch.empty((3, 16)), epilogue=numpy.int64(ops.EPI_ADD))
-    assert len(seen) == 9
-    for name, args in seen:
-        for kind, value in zip(ops._SIGS.get(name) or ops._OPTIONAL_SIGS[name], args):
-            kind.from_param(value)  # what a call through ctypes asks of it
-            assert kind is not ctypes.c_float or value in (0.0, 0.5)
