@@ -58,7 +58,7 @@ __device__ __forceinline__ float int8_bias(const Int8Epilogue& p, uint32_t raw) 
 struct Int8RowScale {
   float a, back;
 };
-__device__ __forceinline__ Int8RowScale int8_row_scale(float sa) { return sa >= I8_FAR ? Int8RowScale{sa * 0x1p-32f, 0x1p32f} : Int8RowScale{sa, 1.0f}; }
+__device__ __forceinline__ Int8RowScale int8_row_scale(float sa) { return fabsf(sa) >= I8_FAR ? Int8RowScale{sa * 0x1p-32f, 0x1p32f} : Int8RowScale{sa, 1.0f}; }
 
 // A sum with its scales and bias. Every kernel rounds here alike (no product joined with an addition), so that a row's outputs have the same
 // bits from all of them.
@@ -192,9 +192,9 @@ __device__ __forceinline__ void int8_outputs(const intx4 (&acc)[RM][CN], int lan
     return v;
   };
   auto outputs = [&](int i, int j) { return scaled(i, j, Int8RowScale{sa[i], 1.0f}); };
-  float most = sa[0];  // of a row's scale in this wave
+  float most = fabsf(sa[0]);  // of a row's scale in this wave
 #pragma unroll
-  for (int i = 1; i < RM; ++i) most = fmaxf(most, sa[i]);
+  for (int i = 1; i < RM; ++i) most = fmaxf(most, fabsf(sa[i]));
   if (!whole || __any(most >= I8_FAR)) {
 #pragma unroll
     for (int i = 0; i < RM; ++i) {

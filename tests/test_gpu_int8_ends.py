@@ -166,6 +166,18 @@ def test_products_of_rows_near_the_largest(ops, monkeypatch, kernel, size, parts
     assert torch.equal(whole[near], ops.gemm_int8(alone, fine, bias=bias))
 
 
+@pytest.mark.parametrize("kernel,size,parts", KERNELS)
+def test_scales_below_zero(ops, monkeypatch, kernel, size, parts):
+    """Rows at hand may have any scale: -s stands for the row of s with its sign turned, near fp32's largest too."""
+    gen = seeded(3)
+    M, N, K = 64 if kernel.endswith("stream") else 150, 203, 1040
+    a, w = ops.quantize_rows(normal(gen, M, K).clamp(-4, 4) * 8e37), ops.quantize_rows(normal(gen, N, K) * 1e-12)
+    monkeypatch.setattr(ops, "_int8_plans", lambda *args: ((0.0, kernel, size, parts),) if kernel else ())
+    want = ops.gemm_int8(a, w, out_dtype=torch.float32)
+    assert torch.isfinite(want).all()
+    assert torch.equal(ops.gemm_int8(ops.Int8Rows(a.q, -a.scale), w, out_dtype=torch.float32), -want)
+
+
 # ------------------------------------------------------------------------------------------------ gates in fp32
 
 
