@@ -11,8 +11,8 @@
 //  * A die takes a run of neighbouring tiles (int8_die_tile).
 //
 // That is the plan of the bf16 product's large tiles (gemm_pingpong.hip): in bytes and clocks an int8 stage of 128 is a bf16 stage of 64,
-// so a product of half the bytes takes half the time. 8,192 x 17,408 x 5,120 gated 1,015 to 1,075 us by card, 2.7 to 2.9 POP/s
-// (a library's 8,192 x 8,192 x 8,192 2.16, this one's 2.86 to 2.95; the matrix cores' peak is nearly twice that): a half stage takes 1,190 clocks of
+// so a product of half the bytes takes half the time. 8,192 x 17,408 x 5,120 gated 1,015 to 1,100 us by card, 2.65 to 2.9 POP/s
+// (a library's 8,192 x 8,192 x 8,192 2.05 to 2.44, this one's 2.3 to 2.95; the matrix cores' peak at 2.4 GHz is 5.0): a half stage takes 1,190 clocks of
 // the 1,024 that its multiplies take alone, at the 1.7 GHz that the chip's power leaves, and of a round's 111,000 clocks 16,000 lie beside its
 // stages (first bytes, outputs).
 //

@@ -70,7 +70,7 @@ __device__ __forceinline__ float int8_output(int sum, Int8RowScale s, float sw, 
 
 // 1 / (1 + exp(-slope x)), SLOPE in millionths, for outputs in fp32: the hardware's exp2 of the rounded exponent, times what the rounding left of it (by itself
 // that is |slope x| halves of a step), so that the exponential and the reciprocal are off by one unit each. The bounds of x change no result (2^x is 0
-// or infinite long before) and keep what is left a number.
+// or infinite long before) and keep what is left a number. us, as for bf16 / so: 64 x 12,288 x 4,096 gated in fp32 23.6 / 24.2, 8,192 x 17,408 x 5,120 1,099 / 1,108.
 template <int SLOPE>
 __device__ __forceinline__ float int8_sigmoid(float x) {
 #pragma clang fp contract(off)

@@ -6,7 +6,8 @@
 //
 // A row of zeros has scale 0 and zeros. A row with a NaN or an infinity has scale NaN and zeros, so that everything computed
 // from it is NaN. Rows whose largest value lies below 2^-100 are multiplied by 2^100 first (exact), where 127 / most
-// could be beyond fp32. Products are rounded to fp32 before they are rounded to whole numbers, as the formula reads.
+// could be beyond fp32. Quotient and products are rounded to fp32 before they are rounded to whole numbers, as the formula reads: an exact half
+// may fall to either side where 127 / most is no fp32 number.
 //
 // Bound by bytes: an entry is read once, and written once in one byte (the norm's h in four more). So a row stays in registers
 // between its reduction and its rounding: eight neighbouring entries to a load (any alignment of an element), J loads to a

@@ -669,7 +669,8 @@ def gemm(a: torch.Tensor, w: torch.Tensor, *, w2: Optional[torch.Tensor] = None,
 class Int8Rows:
     """Rows of 8-bit integers: ``q`` (int8 [n, width], rows contiguous, any distance apart) and one fp32 ``scale`` per row [n]; row r
     stands for ``q[r] * scale[r]``. Activations are such rows by token, a weight [N, K] by output channel. Made by
-    ``quantize_rows`` and ``rmsnorm_int8``, or from tensors at hand, which are looked over here, once, and keep their sizes from then on."""
+    ``quantize_rows`` and ``rmsnorm_int8``, or from tensors at hand, which are looked over here, once, and keep their sizes from then on. ``q``
+    and ``scale`` of rows that the kernels made are views of one allocation, which either keeps alive: clone what is to outlive the other."""
 
     # those that the kernels make are one fp32 allocation (1.3 us on the host, a third of what it does beside a launch): the scales, and the
     # rows from entry `_rows_at` on
@@ -791,8 +792,8 @@ def _new_rows(n: int, width: int, dtype: torch.dtype, beside: torch.Tensor) -> t
 
 
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
-    """Rows of ``x`` (fp32 or bf16 [n, width], any distance apart) as 8-bit integers: scale = max |x| / 127, q = x * (127 / max |x|)
-    rounded to the nearest whole number, halves to even. A row of zeros has scale 0; one with a NaN or an infinity has scale NaN
+    """Rows of ``x`` (fp32 or bf16 [n, width], any distance apart) as 8-bit integers: scale = max |x| / 127, q = x * (127 / max |x|) as fp32 rounds
+    it, made the nearest whole number, halves to even. A row of zeros has scale 0; one with a NaN or an infinity has scale NaN
     and zeros, so that what is computed from it is NaN. For activations in front of ``gemm_int8``, and for a weight [N, K] at load."""
     n, width, distance = _rows_of(x, "quantize_rows input")
     code = _code(x.dtype)
@@ -851,7 +852,7 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, *, w2: Optional[Int8Rows] = None, bias: 
               gate: int = 0, gate_limit: float = 0.0) -> torch.Tensor:
     """out[m, n] = a.scale[m] * w.scale[n] * sum_k a.q[m, k] * w.q[n, k] (+ bias[n]): a product of 8-bit rows with a weight's output
     channels. The sums are whole numbers and exact (up to 131,071 inputs), so a row has the same bits whatever rows stand
-    beside it. Epilogues and gate functions as in ``gemm``: EPI_STORE writes ``out_dtype`` (bf16 where nothing is said), EPI_ADD adds into
+    beside it; the scales are multiplied in that order, with no overflow in between. Epilogues and gate functions as in ``gemm``: EPI_STORE writes ``out_dtype`` (bf16 where nothing is said), EPI_ADD adds into
     the fp32 ``out``, EPI_GATED writes gate(a w + bias, a w2). Rows of any number of entries at any alignment are taken; the fast kernels
     ask for multiples of 16 that begin on 16 bytes."""
     M, K, lda = _int8_rows(a, "gemm_int8 input")
